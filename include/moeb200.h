@@ -510,6 +510,150 @@ int moe_synth_weights(void *y, int64_t n_blocks, int qtype, uint64_t seed, float
                       void *stream);
 int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream);
 
+/* ---- the operators around an expert layer ------------------------------------------
+ * Routing by other rules than softmax + top-k, the norms before and after the
+ * layer with its gate and residual, and low-rank adapters of many requests.
+ * moe_route, moe_block_norm, moe_combine_norm and moe_adapters_apply are
+ * stateless: device pointers on the current device, everything on `stream`,
+ * no workspace, n_tok = 0 does nothing, and all of them can be captured in a
+ * CUDA graph.  moe_block_forward runs them as one expert layer.
+ *
+ * Row strides (ld_*) count elements.  Elements of a row are contiguous. */
+#define MOE_DTYPE_F32  0
+#define MOE_DTYPE_BF16 1
+#define MOE_DTYPE_F16  2
+
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+
+/* A routing rule.  With scores s = softmax(logits) or sigmoid(logits) and
+ * choice values c = s + bias (c = s without bias):
+ *   groups: the experts form n_group groups of n_expert / n_group consecutive
+ *     ones; a group's score is its largest c (group_top 1) or the sum of its
+ *     two largest (group_top 2); the topk_group best groups are kept;
+ *   ids: the k largest c of the kept groups, in order;
+ *   w: s[ids], divided by their sum when renorm (0 where that sum is 0), times
+ *     scale.  The bias decides who is chosen, never the weight.
+ * Ties go to the lower index.  A NaN counts as -inf when experts are compared
+ * and stays NaN in the weights; a softmax over nothing but -inf is 0.  The
+ * comparison is exact: it goes by the logits where c falls with them, else by
+ * c in 64 bits, so that no rounding to 32 bits decides between experts.
+ * Limits: n_expert <= 512, k <= 32, n_group <= 32, a divisor of n_expert;
+ * k <= topk_group * n_expert / n_group.  The reference routes by softmax,
+ * top-k and renormalisation alone (context of patches/0007:101-128), which is
+ * moe_router_run. */
+typedef struct moe_route_cfg {
+    int32_t n_expert, k;
+    int32_t score;             /* MOE_SCORE_*                                   */
+    int32_t n_group;           /* 1: no groups                                  */
+    int32_t topk_group;
+    int32_t group_top;         /* 1 or 2                                        */
+    int32_t renorm;
+    float   scale;
+} moe_route_cfg;
+
+/* ids / w [n_tok][k] from logits [n_tok] rows of stride ld, type dtype; bias
+ * [n_expert] fp32 or NULL. */
+int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype, int64_t ld, int n_tok,
+              const float *bias, int32_t *ids, float *w, void *stream);
+
+/* The rule of one layer of a context (cfg->n_expert and cfg->k the context's;
+ * bias host or device memory, copied) for moe_layer_forward, _path, _noalloc,
+ * moe_ep_route_pack and moe_block_forward; cfg NULL: softmax, top-k and
+ * renormalisation again.  With the cache prior, delta is added to c of resident
+ * experts after the groups are chosen.  moe_decode has the default rule built
+ * in and returns MOE_ERR_UNSUPPORTED while a layer has another.  Synchronous. */
+int moe_set_routing(moe_ctx *ctx, int layer, const moe_route_cfg *cfg, const float *bias);
+
+#define MOE_GATE_NONE    0
+#define MOE_GATE_TOKEN   1     /* one value per row: [n_tok] of stride ld_gate  */
+#define MOE_GATE_CHANNEL 2     /* fp32 [n_embd], the same for every row         */
+#define MOE_GATE_FULL    3     /* [n_tok] rows of n_embd, stride ld_gate        */
+#define MOE_ACT_NONE     0
+#define MOE_ACT_SIGMOID  1
+
+/* The norms around a block:
+ *   z  = y / sqrt(mean(y^2) + eps) * (post + weight_offset)   (z = y without post)
+ *   r' = r + scale * act(gate) * z
+ *   x  = r' / sqrt(mean(r'^2) + eps) * (pre + weight_offset)  (factor 1 without pre)
+ * in fp32, each of r' and x rounded once to its type (x from the unrounded r').
+ * post / pre are fp32 [n_embd] or NULL; weight_offset 1 for weights stored
+ * around 0.  n_embd <= 16384.  Rows of 16-byte-aligned pointers and strides with
+ * n_embd % 8 == 0 take vector loads; others are accepted. */
+typedef struct moe_norm {
+    int32_t      n_embd;
+    int32_t      gate_kind;    /* MOE_GATE_*                                    */
+    int32_t      gate_act;     /* MOE_ACT_*                                     */
+    float        scale, eps, weight_offset;
+    const float *post, *pre;
+    const void  *gate;
+    int64_t      ld_gate;
+} moe_norm;
+
+/* r, r_out [n_tok][n_embd] of r_dtype; y, x and a token or full gate of dtype.
+ * r_dtype is MOE_DTYPE_F32 or dtype.  y NULL: r' = r (then no post, no gate).
+ * r_out NULL (r' not wanted) or x NULL (no second norm), not both.  r_out may be
+ * r, and x may be y. */
+int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r, const void *y, int dtype,
+                   int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok, void *stream);
+
+/* The same with y[t] = sum over j in order of w[t][j] * y_rows[pos[t][j]], then
+ * + add[t] when given: moe_ep_combine's sum, bit for bit, never written to
+ * memory.  All fp32; pos / w [n_tok][k], add [n_tok][n_embd].  A pos outside
+ * [0, n_rows) adds nothing (-1: an empty pair). */
+int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const float *y_rows, int64_t ld_rows,
+                     int n_rows, const int32_t *pos, const float *w, int k, const float *add, float *r_out,
+                     int64_t ld_ro, float *x, int64_t ld_x, int n_tok, void *stream);
+
+/* Low-rank adapters of one projection n_in -> n_out, in 16 bits.  Adapter i:
+ * A = a + i * rank * lda, rank rows of stride lda (a multiple of 8, columns from
+ * n_in on zero); B = b + i * n_out * rank, n_out rows of rank.  rank is a
+ * multiple of 8, <= 128; ranks[i] <= rank is how much of adapter i is used (what
+ * lies beyond is never used; NULL: all).  a and b are 16-byte aligned.
+ * n_in <= 16384.  ggml applies adapters beside a projection in build_lora_mm,
+ * which build_moe_ffn calls for the router (context of patches/0007:101-128);
+ * there all tokens share them. */
+typedef struct moe_adapters {
+    const void    *a, *b;
+    const float   *scale;      /* [n_adapters]                                  */
+    const int32_t *ranks;      /* [n_adapters] or NULL                          */
+    int32_t        n_adapters, rank, n_in, n_out;
+    int32_t        dtype;      /* of a and b: MOE_DTYPE_BF16 or MOE_DTYPE_F16   */
+    int64_t        lda;
+} moe_adapters;
+
+/* out[t] = y[t] + scale[i] * B_i (A_i x[t]) with i = ids[t] (device); y NULL
+ * counts as 0, out may be y.  A row whose id is outside [0, n_adapters) gets
+ * y[t] (-1: a request without an adapter).  Types: x fp32, y and out fp32; or x
+ * of the weights' type, y and out of that type or fp32.  A x stays in fp32. */
+int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *x, int x_dtype, int64_t ld_x,
+                       const void *y, int64_t ld_y, void *out, int out_dtype, int64_t ld_out, int n_tok,
+                       void *stream);
+
+/* One expert layer with what is around it, for n_tok tokens: x [n_tok][n_embd]
+ * (the pre-norm's output) -> router logits, + router_adapters' -> the layer's
+ * routing rule -> experts -> combine, + adapters' -> the norms.
+ *   norm NULL: y [n_tok][n_embd] gets the layer's output, as moe_layer_forward;
+ *   norm given: y is NULL, and with the residual r [n_tok][n_embd], r_out and
+ *   x_out (either may be NULL, not both; r_out may be r, and x_out may be x) get
+ *   moe_combine_norm's r' and x: the input of the next block.  x_out != r_out.
+ * adapter_ids [n_tok] (device) choose both kinds' adapters.  Everything is fp32
+ * contiguous; a token or full gate too.  ids / w are optional outputs; path,
+ * prior, observation and callbacks are moe_layer_forward_path's.  Without
+ * adapters, ids, w and y are its bits.  The context's scratch grows with n_tok
+ * as there: one stream at a time per context, and the largest n_tok once before
+ * any call is captured in a CUDA graph. */
+typedef struct moe_block {
+    const moe_adapters *router_adapters;   /* n_embd -> n_expert, or NULL       */
+    const moe_adapters *adapters;          /* n_embd -> n_embd, or NULL         */
+    const int32_t      *adapter_ids;
+    const moe_norm     *norm;              /* n_embd the context's, or NULL     */
+    const float        *r;
+    float              *r_out, *x_out;
+} moe_block;
+int moe_block_forward(moe_ctx *ctx, int layer, const float *x, int n_tok, const moe_block *b, float *y,
+                      int32_t *ids, float *w, int path, void *stream);
+
 /* ---- ExpertCache (src/prefetch_engine.py:45-168) ----------------------------------- */
 
 typedef struct moe_xc moe_xc;

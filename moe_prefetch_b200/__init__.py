@@ -16,6 +16,9 @@ def __getattr__(name):
     if name in ("MoeStack", "expert_bytes", "load_heat", "save_heat"):
         from . import stack
         return getattr(stack, name)
+    if name in ("Routing", "BlockNorm", "AdapterSet"):
+        from . import block
+        return getattr(block, name)
     if name in ("ExpertCache", "EXPERT_BYTES", "EXPERT_MIB"):
         from . import prefetch_engine
         return getattr(prefetch_engine, name)

@@ -62,6 +62,33 @@ class MoeDecodeDbg(C.Structure):
                 ("prof", C.c_void_p), ("starve", C.c_int32), ("spec", C.c_int32)]
 
 
+class MoeRouteCfg(C.Structure):
+    """struct moe_route_cfg."""
+    _fields_ = [("n_expert", C.c_int32), ("k", C.c_int32), ("score", C.c_int32), ("n_group", C.c_int32),
+                ("topk_group", C.c_int32), ("group_top", C.c_int32), ("renorm", C.c_int32), ("scale", C.c_float)]
+
+
+class MoeNorm(C.Structure):
+    """struct moe_norm."""
+    _fields_ = [("n_embd", C.c_int32), ("gate_kind", C.c_int32), ("gate_act", C.c_int32), ("scale", C.c_float),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("post", C.c_void_p), ("pre", C.c_void_p),
+                ("gate", C.c_void_p), ("ld_gate", C.c_int64)]
+
+
+class MoeAdapters(C.Structure):
+    """struct moe_adapters."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("ranks", C.c_void_p),
+                ("n_adapters", C.c_int32), ("rank", C.c_int32), ("n_in", C.c_int32), ("n_out", C.c_int32),
+                ("dtype", C.c_int32), ("lda", C.c_int64)]
+
+
+class MoeBlock(C.Structure):
+    """struct moe_block."""
+    _fields_ = [("router_adapters", C.POINTER(MoeAdapters)), ("adapters", C.POINTER(MoeAdapters)),
+                ("adapter_ids", C.c_void_p), ("norm", C.POINTER(MoeNorm)), ("r", C.c_void_p),
+                ("r_out", C.c_void_p), ("x_out", C.c_void_p)]
+
+
 P = C.c_void_p
 I = C.c_int
 I64 = C.c_int64
@@ -105,6 +132,12 @@ SIGNATURES = {
     "moe_set_evictor": (I, [P, I, P, I, P, P, P, P]),
     "moe_warm_start": (I, [P, P]),
     "moe_router_run": (I, [P, P, I, I, I, P, I, F, I, P, P, P, P]),
+    "moe_route": (I, [P, P, I, I64, I, P, P, P, P]),
+    "moe_set_routing": (I, [P, I, P, P]),
+    "moe_block_norm": (I, [P, P, I, I64, P, I, I64, P, I64, P, I64, I, P]),
+    "moe_combine_norm": (I, [P, P, I64, P, I64, I, P, P, I, P, P, I64, P, I64, I, P]),
+    "moe_adapters_apply": (I, [P, P, P, I, I64, P, I64, P, I, I64, I, P]),
+    "moe_block_forward": (I, [P, I, P, I, P, P, P, P, I, P]),
     "moe_quantize": (I, [P, P, I64, I, P]),
     "moe_synth_weights": (I, [P, I64, I, C.c_uint64, F, P]),
     "moe_synth_f32": (I, [P, I64, C.c_uint64, F, P]),

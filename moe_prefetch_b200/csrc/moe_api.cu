@@ -32,6 +32,8 @@ struct LayerMem {
     uint8_t *shared = nullptr;        // shared expert: gate | up | down (n_shared == 1)
     uint8_t *sgate = nullptr, *sup = nullptr, *sdown = nullptr;
     bool shared_set = false;
+    bool ruled = false;               // a routing rule other than the default (moe_set_routing)
+    RouteSpec rule{};
 };
 
 }  // namespace
@@ -79,6 +81,11 @@ struct moe_ctx {
     float *ep_y = nullptr;             // [world * cap][n_embd]
     unsigned long long *ep_epoch = nullptr;   // [0] the exchange epoch, [1] the push kernel's CTA count
     bool ep_connected = false;
+    float *route_bias = nullptr;       // [L][E], allocated by the first moe_set_routing with a bias
+    // moe_block_forward: router logits [n_tok][E] with router adapters, the
+    // adapters' rows [n_tok][H]
+    float *s_block = nullptr;
+    size_t s_block_cap = 0;            // floats
     // tensor-core GEMM operand tiles (fp16)
     void *s_gemm = nullptr;
     int s_gemm_cap_tok = 0;
@@ -469,6 +476,8 @@ extern "C" void moe_destroy(moe_ctx *c) {
     cudaFree(c->s_group);
     cudaFree(c->s_ypair);
     cudaFree(c->s_gemm);
+    cudaFree(c->route_bias);
+    cudaFree(c->s_block);
     if (c->h_jobs) cudaFreeHost(c->h_jobs);
     if (c->ev_step) cudaEventDestroy(c->ev_step);
     if (c->ev_copy) cudaEventDestroy(c->ev_copy);
@@ -698,6 +707,31 @@ static int expert_pairs(moe_ctx *c, const int32_t *ids, const float *w, int n_to
     return MOE_OK;
 }
 
+// Route n_tok tokens by the layer's rule.  `cached`: with the cache prior and
+// the observation of a single token (expert-parallel routing has neither).
+// `logits` (with router adapters): the finished logits, instead of x.
+static cudaError_t route_tokens(moe_ctx *c, int layer, const float *x, int n_tok, int32_t *ids, float *w,
+                                cudaStream_t s, bool cached = true, const float *logits = nullptr) {
+    const moe_cfg &g = c->cfg;
+    const LayerMem &m = c->L[layer];
+    const float *W = c->router + (size_t)layer * g.n_expert * g.n_embd;
+    const int32_t *table = c->st.table + (size_t)layer * g.n_expert;
+    const bool one = cached && n_tok == 1;
+    const float delta = cached ? g.cache_prior : 0.0f;
+    const int prior = one && g.cache_prior > 0.0f, obs = one ? layer : -1;
+    const int32_t *pub = cached ? c->st.slot_expert + c->slot_off[layer] : nullptr;
+    if (logits) {
+        const RouteSpec sp = m.ruled ? m.rule : route_spec(g.n_expert, g.n_used, 0, 1, 1, 1, 1, 1.0f, nullptr);
+        return launch_route(sp, logits, DT_F32, g.n_expert, n_tok, ids, w, table, m.ns, delta, prior, &c->st, obs,
+                            pub, s);
+    }
+    if (m.ruled)
+        return launch_router_rule(W, x, n_tok, g.n_embd, m.rule, table, m.ns, delta, prior, ids, w, &c->st, obs, pub,
+                                  s);
+    return launch_router(W, x, n_tok, g.n_expert, g.n_embd, table, m.ns, delta, prior, g.n_used, ids, w, nullptr,
+                         &c->st, obs, pub, s);
+}
+
 static int check_shared(moe_ctx *c, int layer) {
     if (c->cfg.n_shared && !c->L[layer].shared_set)
         return fail(c, MOE_ERR_STATE, "the shared expert of layer %d is not set", layer);
@@ -911,11 +945,7 @@ extern "C" int moe_layer_forward(moe_ctx *c, int layer, const float *x, float *y
     if (g.stream && n_tok == 1 && (r = stream_enter(c, layer, s)) != MOE_OK) return r;
     int32_t *ids_d = ids ? ids : c->s_ids;
     float *w_d = w ? w : c->s_w;
-    const int32_t *table = c->st.table + (size_t)layer * g.n_expert;
-    CK(launch_router(c->router + (size_t)layer * g.n_expert * g.n_embd, x, n_tok, g.n_expert, g.n_embd,
-                     table, c->L[layer].ns, g.cache_prior, n_tok == 1 && g.cache_prior > 0.0f, g.n_used,
-                     ids_d, w_d, nullptr, &c->st, n_tok == 1 ? layer : -1,
-                     c->st.slot_expert + c->slot_off[layer], s));
+    CK(route_tokens(c, layer, x, n_tok, ids_d, w_d, s));
     const int32_t *ids_e;
     const float *w_e;
     int kx;
@@ -966,11 +996,7 @@ extern "C" int moe_layer_forward_path(moe_ctx *c, int layer, const float *x, flo
     if (g.stream && n_tok == 1 && (r = stream_enter(c, layer, s)) != MOE_OK) return r;
     int32_t *ids_d = ids ? ids : c->s_ids;
     float *w_d = w ? w : c->s_w;
-    const int32_t *table = c->st.table + (size_t)layer * g.n_expert;
-    CK(launch_router(c->router + (size_t)layer * g.n_expert * g.n_embd, x, n_tok, g.n_expert, g.n_embd,
-                     table, c->L[layer].ns, g.cache_prior, n_tok == 1 && g.cache_prior > 0.0f, g.n_used,
-                     ids_d, w_d, nullptr, &c->st, n_tok == 1 ? layer : -1,
-                     c->st.slot_expert + c->slot_off[layer], s));
+    CK(route_tokens(c, layer, x, n_tok, ids_d, w_d, s));
     const int32_t *ids_e;
     const float *w_e;
     int kx;
@@ -1000,9 +1026,7 @@ extern "C" int moe_ep_route_pack(moe_ctx *c, int layer, const float *x, int n_to
     const int r = ensure_scratch(c, n_tok);
     if (r != MOE_OK) return r;
     cudaStream_t s = (cudaStream_t)stream;
-    const int32_t *table = c->st.table + (size_t)layer * g.n_expert;
-    CK(launch_router(c->router + (size_t)layer * g.n_expert * g.n_embd, x, n_tok, g.n_expert, g.n_embd,
-                     table, c->L[layer].ns, 0.0f, 0, g.n_used, ids, w, nullptr, &c->st, -1, nullptr, s));
+    CK(route_tokens(c, layer, x, n_tok, ids, w, s, false));
     GroupBufs gg = c->grp;
     gg.cnt = send_count;
     gg.pair_pos = pos;
@@ -1268,11 +1292,7 @@ extern "C" int moe_layer_forward_noalloc(moe_ctx *c, int layer, const float *x, 
     float *w_d = w ? w : reinterpret_cast<float *>(scr + sel);
     float *act = reinterpret_cast<float *>(scr + 2 * sel);
     cudaStream_t s = (cudaStream_t)stream;
-    const int32_t *table = c->st.table + (size_t)layer * g.n_expert;
-    CK(launch_router(c->router + (size_t)layer * g.n_expert * g.n_embd, x, n_tok, g.n_expert, g.n_embd,
-                     table, c->L[layer].ns, g.cache_prior, n_tok == 1 && g.cache_prior > 0.0f, g.n_used,
-                     ids_d, w_d, nullptr, &c->st, n_tok == 1 ? layer : -1,
-                     c->st.slot_expert + c->slot_off[layer], s));
+    CK(route_tokens(c, layer, x, n_tok, ids_d, w_d, s));
     CK(launch_experts(make_src(c, layer), x, ids_d, w_d, n_tok, g.n_used, g.n_embd, g.n_ff,
                       g.down_type, act, nullptr, y, c->err, s));
     return MOE_OK;
@@ -1286,6 +1306,9 @@ extern "C" int moe_decode(moe_ctx *c, const float *h, float *out, int n_tok,
         if (r != MOE_OK) return r;
     }
     CK(cudaSetDevice(c->cfg.device));
+    for (int l = 0; l < c->cfg.n_layers; ++l)
+        if (c->L[l].ruled)
+            return fail(c, MOE_ERR_UNSUPPORTED, "moe_decode: layer %d has a routing rule (moe_set_routing)", l);
     if (c->dp.smem_bytes > 227 * 1024)
         return fail(c, MOE_ERR_UNSUPPORTED, "decode needs %d bytes of shared memory", c->dp.smem_bytes);
     cudaStream_t s = (cudaStream_t)stream;
@@ -1688,6 +1711,286 @@ extern "C" int moe_decode_info(const moe_ctx *c, int32_t *out, int n) {
     const int32_t v[] = {c->grid, c->dp.smem_bytes, c->dp.gu_rows_max, c->dp.dn_rows_max, 512};
     for (int i = 0; i < n && i < 5; ++i) out[i] = v[i];
     return MOE_OK;
+}
+
+// ---------------------------------------------------------------------------
+// the operators around an expert layer
+// ---------------------------------------------------------------------------
+
+// What is wrong with a routing rule (null: nothing).
+static const char *route_bad(const moe_route_cfg &r, int *code) {
+    *code = MOE_ERR_ARG;
+    if (r.n_expert <= 0 || r.k <= 0 || r.n_group <= 0 || r.topk_group <= 0) return "a non-positive size";
+    if (r.score != MOE_SCORE_SOFTMAX && r.score != MOE_SCORE_SIGMOID) return "an unknown score";
+    if (r.group_top != 1 && r.group_top != 2) return "group_top must be 1 or 2";
+    if (r.n_expert % r.n_group) return "n_group does not divide n_expert";
+    if (r.topk_group > r.n_group) return "topk_group is above n_group";
+    if ((int64_t)r.k > (int64_t)r.topk_group * (r.n_expert / r.n_group)) return "k is above the experts of the kept groups";
+    *code = MOE_ERR_UNSUPPORTED;
+    if (r.n_expert > ROUTE_MAX_EXPERT) return "n_expert is above 512";
+    if (r.k > ROUTE_MAX_K) return "k is above 32";
+    if (r.n_group > ROUTE_MAX_GROUP) return "n_group is above 32";
+    return nullptr;
+}
+
+static bool dtype_ok(int d) { return d == MOE_DTYPE_F32 || d == MOE_DTYPE_BF16 || d == MOE_DTYPE_F16; }
+
+extern "C" int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype, int64_t ld, int n_tok,
+                         const float *bias, int32_t *ids, float *w, void *stream) {
+    moe_ctx *c = nullptr;
+    if (!cfg || n_tok < 0 || !dtype_ok(dtype) || (n_tok && (!logits || !ids || !w)))
+        return fail(c, MOE_ERR_ARG, "moe_route: bad argument");
+    int code;
+    if (const char *m = route_bad(*cfg, &code)) return fail(c, code, "moe_route: %s", m);
+    if (ld < cfg->n_expert) return fail(c, MOE_ERR_ARG, "moe_route: the row stride is below n_expert");
+    if (!n_tok) return MOE_OK;
+    CK(launch_route(route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
+                               cfg->renorm, cfg->scale, bias),
+                    logits, dtype, ld, n_tok, ids, w, nullptr, 0, 0.0f, 0, nullptr, -1, nullptr,
+                    (cudaStream_t)stream));
+    return MOE_OK;
+}
+
+extern "C" int moe_set_routing(moe_ctx *c, int layer, const moe_route_cfg *cfg, const float *bias) {
+    if (!c || layer < 0 || layer >= c->cfg.n_layers) return fail(c, MOE_ERR_ARG, "moe_set_routing: bad argument");
+    LayerMem &m = c->L[layer];
+    const moe_cfg &g = c->cfg;
+    if (!cfg) {
+        m.ruled = false;
+        return MOE_OK;
+    }
+    int code;
+    if (const char *w = route_bad(*cfg, &code)) return fail(c, code, "moe_set_routing: %s", w);
+    if (cfg->n_expert != g.n_expert || cfg->k != g.n_used)
+        return fail(c, MOE_ERR_ARG, "moe_set_routing: %d experts, top %d; the context has %d and %d", cfg->n_expert,
+                    cfg->k, g.n_expert, g.n_used);
+    CK(cudaSetDevice(g.device));
+    float *dst = nullptr;
+    if (bias) {
+        if (!c->route_bias &&
+            cudaMalloc(&c->route_bias, sizeof(float) * (size_t)g.n_layers * g.n_expert) != cudaSuccess) {
+            c->route_bias = nullptr;
+            return fail(c, MOE_ERR_OOM, "moe_set_routing: the bias allocation failed");
+        }
+        dst = c->route_bias + (size_t)layer * g.n_expert;
+        CK(cudaDeviceSynchronize());   // no kernel reads the old bias
+        CK(cudaMemcpy(dst, bias, sizeof(float) * g.n_expert, cudaMemcpyDefault));
+        CK(cudaDeviceSynchronize());
+    }
+    m.rule = route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
+                        cfg->renorm, cfg->scale, dst);
+    m.ruled = true;
+    return MOE_OK;
+}
+
+// What is wrong with a norm of n_tok rows (null: nothing).
+static const char *norm_bad(const moe_norm &n, int n_tok, int *code) {
+    *code = MOE_ERR_ARG;
+    if (n.n_embd <= 0 || n_tok < 0) return "a bad size";
+    if (n.gate_kind < MOE_GATE_NONE || n.gate_kind > MOE_GATE_FULL) return "an unknown gate kind";
+    if (n.gate_act != MOE_ACT_NONE && n.gate_act != MOE_ACT_SIGMOID) return "an unknown gate activation";
+    if (n_tok && n.gate_kind != MOE_GATE_NONE && !n.gate) return "the gate is missing";
+    if (n.gate_kind == MOE_GATE_FULL && n.ld_gate < n.n_embd) return "the gate's row stride is below n_embd";
+    if (n.gate_kind == MOE_GATE_TOKEN && n.ld_gate < 0) return "the gate's stride is negative";
+    *code = MOE_ERR_UNSUPPORTED;
+    if (n.n_embd > NORM_MAX_EMBD) return "n_embd is above 16384";
+    return nullptr;
+}
+
+static NormArgs norm_args(const moe_norm &n, int n_tok) {
+    NormArgs a{};
+    a.n_tok = n_tok; a.n_embd = n.n_embd;
+    a.post = n.post; a.pre = n.pre;
+    a.gate = n.gate; a.ld_gate = n.ld_gate; a.gate_kind = n.gate_kind; a.sigmoid = n.gate_act == MOE_ACT_SIGMOID;
+    a.scale = n.scale; a.eps = n.eps; a.offset = n.weight_offset;
+    return a;
+}
+
+extern "C" int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r, const void *y, int dtype,
+                              int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok,
+                              void *stream) {
+    moe_ctx *c = nullptr;
+    if (!nm || !dtype_ok(r_dtype) || !dtype_ok(dtype) || (r_dtype != MOE_DTYPE_F32 && r_dtype != dtype))
+        return fail(c, MOE_ERR_ARG, "moe_block_norm: bad argument");
+    int code;
+    if (const char *m = norm_bad(*nm, n_tok, &code)) return fail(c, code, "moe_block_norm: %s", m);
+    if (!n_tok) return MOE_OK;
+    if (!r || (!r_out && !x)) return fail(c, MOE_ERR_ARG, "moe_block_norm: r, or both outputs, are missing");
+    if (!y && (nm->post || nm->gate_kind != MOE_GATE_NONE))
+        return fail(c, MOE_ERR_ARG, "moe_block_norm: a post norm or gate needs y");
+    if (ld_r < nm->n_embd || (y && ld_y < nm->n_embd) || (r_out && ld_ro < nm->n_embd) || (x && ld_x < nm->n_embd))
+        return fail(c, MOE_ERR_ARG, "moe_block_norm: a row stride is below n_embd");
+    if (r_out && r_out == x) return fail(c, MOE_ERR_ARG, "moe_block_norm: r_out and x are the same");
+    NormArgs a = norm_args(*nm, n_tok);
+    a.r = r; a.ld_r = ld_r;
+    a.y = y; a.ld_y = ld_y;
+    a.r_out = r_out; a.ld_ro = ld_ro;
+    a.x = x; a.ld_x = ld_x;
+    CK(launch_block_norm(a, r_dtype, dtype, (cudaStream_t)stream));
+    return MOE_OK;
+}
+
+extern "C" int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const float *y_rows,
+                                int64_t ld_rows, int n_rows, const int32_t *pos, const float *w, int k,
+                                const float *add, float *r_out, int64_t ld_ro, float *x, int64_t ld_x, int n_tok,
+                                void *stream) {
+    moe_ctx *c = nullptr;
+    if (!nm || k <= 0 || n_rows < 0) return fail(c, MOE_ERR_ARG, "moe_combine_norm: bad argument");
+    int code;
+    if (const char *m = norm_bad(*nm, n_tok, &code)) return fail(c, code, "moe_combine_norm: %s", m);
+    if (!n_tok) return MOE_OK;
+    if (!r || (n_rows && !y_rows) || !pos || !w || (!r_out && !x))
+        return fail(c, MOE_ERR_ARG, "moe_combine_norm: an input, or both outputs, are missing");
+    if (ld_r < nm->n_embd || ld_rows < nm->n_embd || (r_out && ld_ro < nm->n_embd) || (x && ld_x < nm->n_embd))
+        return fail(c, MOE_ERR_ARG, "moe_combine_norm: a row stride is below n_embd");
+    if (r_out && r_out == x) return fail(c, MOE_ERR_ARG, "moe_combine_norm: r_out and x are the same");
+    NormArgs a = norm_args(*nm, n_tok);
+    a.r = r; a.ld_r = ld_r;
+    a.y = y_rows; a.ld_y = ld_rows; a.n_rows = n_rows;
+    a.pos = pos; a.w = w; a.k = k; a.add = add;
+    a.r_out = r_out; a.ld_ro = ld_ro;
+    a.x = x; a.ld_x = ld_x;
+    CK(launch_block_norm(a, DT_F32, DT_F32, (cudaStream_t)stream));
+    return MOE_OK;
+}
+
+// What is wrong with a set of adapters for n_tok tokens (null: nothing).
+static const char *adapters_bad(const moe_adapters &s, int n_tok, int *code) {
+    *code = MOE_ERR_ARG;
+    if (s.n_adapters <= 0 || s.rank <= 0 || s.n_in <= 0 || s.n_out <= 0 || n_tok < 0) return "a non-positive size";
+    if (s.dtype != MOE_DTYPE_BF16 && s.dtype != MOE_DTYPE_F16) return "the weights must be bf16 or fp16";
+    if (!s.a || !s.b || !s.scale) return "a weight is missing";
+    if (s.rank % 8 || s.lda % 8 || s.lda < s.n_in) return "rank and lda must be multiples of 8, lda at least n_in";
+    if (((uintptr_t)s.a | (uintptr_t)s.b) & 15) return "the weights must be 16-byte aligned";
+    *code = MOE_ERR_UNSUPPORTED;
+    if (s.rank > ADAPTER_MAX_RANK) return "rank is above 128";
+    if (s.n_in > ADAPTER_MAX_IN) return "n_in is above 16384";
+    return nullptr;
+}
+
+static AdapterArgs adapter_args(const moe_adapters &s, const int32_t *ids, int n_tok) {
+    AdapterArgs p{};
+    p.n_tok = n_tok; p.n_in = s.n_in; p.n_out = s.n_out; p.n_adapters = s.n_adapters; p.rank = s.rank;
+    p.a = s.a; p.b = s.b; p.lda = s.lda; p.scale = s.scale; p.ranks = s.ranks; p.ids = ids;
+    return p;
+}
+
+extern "C" int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *x, int x_dtype,
+                                  int64_t ld_x, const void *y, int64_t ld_y, void *out, int out_dtype,
+                                  int64_t ld_out, int n_tok, void *stream) {
+    moe_ctx *c = nullptr;
+    if (!set) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: bad argument");
+    int code;
+    if (const char *m = adapters_bad(*set, n_tok, &code)) return fail(c, code, "moe_adapters_apply: %s", m);
+    if (!(x_dtype == MOE_DTYPE_F32 && out_dtype == MOE_DTYPE_F32) &&
+        !(x_dtype == set->dtype && (out_dtype == set->dtype || out_dtype == MOE_DTYPE_F32)))
+        return fail(c, MOE_ERR_ARG, "moe_adapters_apply: types x %d, weights %d, out %d", x_dtype, set->dtype, out_dtype);
+    if (!n_tok) return MOE_OK;
+    if (!ids || !x || !out) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: a pointer is missing");
+    if (ld_x < set->n_in || (y && ld_y < set->n_out) || ld_out < set->n_out)
+        return fail(c, MOE_ERR_ARG, "moe_adapters_apply: a row stride is below the row");
+    if (y == out && ld_y != ld_out) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: y and out share memory with two strides");
+    AdapterArgs p = adapter_args(*set, ids, n_tok);
+    p.x = x; p.ld_x = ld_x;
+    p.y = y; p.ld_y = ld_y;
+    p.out = out; p.ld_out = ld_out;
+    CK(launch_adapters(p, x_dtype, set->dtype, out_dtype, (cudaStream_t)stream));
+    return MOE_OK;
+}
+
+extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_tok, const moe_block *b, float *y,
+                                 int32_t *ids, float *w, int path, void *stream) {
+    if (!c || !b || n_tok < 0 || (n_tok && !x) || layer < 0 || layer >= c->cfg.n_layers)
+        return fail(c, MOE_ERR_ARG, "moe_block_forward: bad argument");
+    const moe_cfg &g = c->cfg;
+    const int H = g.n_embd, E = g.n_expert;
+    const moe_adapters *ra = b->router_adapters, *la = b->adapters;
+    int code;
+    for (const moe_adapters *s : {ra, la}) {
+        if (!s) continue;
+        if (const char *m = adapters_bad(*s, n_tok, &code)) return fail(c, code, "moe_block_forward: adapters: %s", m);
+        if (s->n_in != H || s->n_out != (s == ra ? E : H))
+            return fail(c, MOE_ERR_ARG, "moe_block_forward: adapters of %d -> %d beside %d -> %d", s->n_in, s->n_out, H,
+                        s == ra ? E : H);
+    }
+    if (n_tok && (ra || la) && !b->adapter_ids) return fail(c, MOE_ERR_ARG, "moe_block_forward: adapter_ids is missing");
+    if (b->norm) {
+        if (const char *m = norm_bad(*b->norm, n_tok, &code)) return fail(c, code, "moe_block_forward: norm: %s", m);
+        if (b->norm->n_embd != H) return fail(c, MOE_ERR_ARG, "moe_block_forward: a norm of %d beside n_embd %d", b->norm->n_embd, H);
+        if (n_tok && (y || !b->r || b->r_out == b->x_out))   // (both null are equal too)
+            return fail(c, MOE_ERR_ARG, "moe_block_forward: a norm takes r and gives r_out and x_out, not y");
+    } else if (n_tok && (!y || b->r || b->r_out || b->x_out)) {
+        return fail(c, MOE_ERR_ARG, "moe_block_forward: without a norm there is y, and no r, r_out, x_out");
+    }
+    const bool gemm_ok = g.down_type == MOE_QTYPE_Q6_K && g.n_ff % 128 == 0 && H % 128 == 0;
+    if (path == MOE_PATH_AUTO)
+        path = gemm_ok && (int64_t)n_tok * g.n_used >= 4 * (int64_t)E ? MOE_PATH_GEMM : MOE_PATH_GEMV;
+    if (path != MOE_PATH_GEMV && path != MOE_PATH_GEMM)
+        return fail(c, MOE_ERR_ARG, "moe_block_forward: unknown path %d", path);
+    if (path == MOE_PATH_GEMM && !gemm_ok)
+        return fail(c, MOE_ERR_UNSUPPORTED, "the GEMM path needs Q6_K down weights and n_ff, n_embd multiples of 128");
+    int rc = check_shared(c, layer);
+    if (rc != MOE_OK || !n_tok) return rc;
+    CK(cudaSetDevice(g.device));
+    if ((rc = ensure_scratch(c, n_tok)) != MOE_OK) return rc;
+    if (path == MOE_PATH_GEMM && (rc = ensure_gemm_scratch(c, n_tok)) != MOE_OK) return rc;
+    const bool add_rows = la && b->norm;   // without a norm the adapters add to y itself
+    const size_t need = (ra ? (size_t)n_tok * E : 0) + (add_rows ? (size_t)n_tok * H : 0);
+    if (need > c->s_block_cap) {
+        cudaFree(c->s_block);
+        c->s_block = nullptr;
+        c->s_block_cap = 0;
+        if (cudaMalloc(&c->s_block, sizeof(float) * need) != cudaSuccess)
+            return fail(c, MOE_ERR_OOM, "moe_block_forward: scratch for %d tokens failed", n_tok);
+        c->s_block_cap = need;
+    }
+    float *logits = ra ? c->s_block : nullptr;
+    float *delta = add_rows ? c->s_block + (ra ? (size_t)n_tok * E : 0) : nullptr;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (g.stream && n_tok == 1 && (rc = stream_enter(c, layer, s)) != MOE_OK) return rc;
+    int32_t *ids_d = ids ? ids : c->s_ids;
+    float *w_d = w ? w : c->s_w;
+    if (ra) {
+        CK(launch_router_logits(c->router + (size_t)layer * E * H, x, n_tok, E, H, logits, s));
+        AdapterArgs p = adapter_args(*ra, b->adapter_ids, n_tok);
+        p.x = x; p.ld_x = H;
+        p.y = logits; p.ld_y = E;
+        p.out = logits; p.ld_out = E;
+        CK(launch_adapters(p, DT_F32, ra->dtype, DT_F32, s));
+    }
+    CK(route_tokens(c, layer, x, n_tok, ids_d, w_d, s, true, logits));
+    const int32_t *ids_e;
+    const float *w_e;
+    int kx;
+    if ((rc = expert_pairs(c, ids_d, w_d, n_tok, s, &ids_e, &w_e, &kx)) != MOE_OK) return rc;
+    CK(launch_group(ids_e, n_tok * kx, E + g.n_shared, path == MOE_PATH_GEMM ? GM_NT : GROUP_TILE, c->grp, c->err, s));
+    if (path == MOE_PATH_GEMM)
+        CK(launch_experts_gemm(make_src(c, layer), x, c->grp, n_tok, kx, H, g.n_ff, g.down_type, w_e, c->s_gemm,
+                               c->s_ypair, nullptr, y, c->err, s));
+    else
+        CK(launch_experts_grouped(make_src(c, layer), x, c->grp, n_tok, kx, H, g.n_ff, g.down_type, w_e, c->s_act,
+                                  c->s_ypair, nullptr, y, c->err, s));
+    if (la) {
+        AdapterArgs p = adapter_args(*la, b->adapter_ids, n_tok);
+        p.x = x; p.ld_x = H;
+        p.y = y; p.ld_y = H;
+        p.out = y ? y : delta; p.ld_out = H;
+        CK(launch_adapters(p, DT_F32, la->dtype, DT_F32, s));
+    }
+    // the lookahead of a streaming context reads x, which x_out may overwrite
+    if (b->norm) {
+        NormArgs a = norm_args(*b->norm, n_tok);
+        a.r = b->r; a.ld_r = H;
+        a.y = c->s_ypair; a.ld_y = H; a.n_rows = n_tok * kx;
+        a.pos = c->grp.pair_pos; a.w = w_e; a.k = kx; a.add = delta;
+        a.r_out = b->r_out; a.ld_ro = H;
+        a.x = b->x_out; a.ld_x = H;
+        const bool ahead = n_tok == 1 && g.stream && b->x_out == x;
+        if (ahead && (rc = after_observe(c, layer, ids_d, g.n_used, s, x)) != MOE_OK) return rc;
+        CK(launch_block_norm(a, DT_F32, DT_F32, s));
+        if (ahead) return MOE_OK;
+    }
+    return n_tok == 1 ? after_observe(c, layer, ids_d, g.n_used, s, x) : MOE_OK;
 }
 
 // ---------------------------------------------------------------------------

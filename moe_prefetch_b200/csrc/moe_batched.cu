@@ -577,7 +577,7 @@ cudaError_t launch_experts_grouped(const ExpertSrc &src, const float *x, const G
         src, aq, ad, as, g.off, g.cnt, g.tiles, g.n_tiles, n_embd, n_ff, down_type, dn_rows, ypair, g.pos_pair,
         direct ? y : nullptr, err);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return direct ? cudaSuccess : launch_combine(ypair, g.pair_pos, w, n_tok, k, n_embd, resid, y, s);
+    return direct || !y ? cudaSuccess : launch_combine(ypair, g.pair_pos, w, n_tok, k, n_embd, resid, y, s);
 }
 
 cudaError_t launch_combine(const float *ypair, const int32_t *pair_pos, const float *w, int n_tok,

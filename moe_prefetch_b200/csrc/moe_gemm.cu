@@ -1061,7 +1061,7 @@ cudaError_t launch_experts_gemm(const ExpertSrc &src, const float *x, const Grou
             err);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return direct ? cudaSuccess : launch_combine(ypair, g.pair_pos, w, n_tok, k, n_embd, resid, y, s);
+    return direct || !y ? cudaSuccess : launch_combine(ypair, g.pair_pos, w, n_tok, k, n_embd, resid, y, s);
 }
 
 }  // namespace moe

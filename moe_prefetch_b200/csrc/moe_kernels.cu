@@ -213,6 +213,11 @@ __global__ void __launch_bounds__(512) k_router(const float *__restrict__ W,
 // batches (the router rows are reused over more tokens), and TOK = 4 with
 // 16 warps, one router row each, for small ones (twice the clusters, and a
 // warp's serial chain of row load and dots is a quarter as long).
+// MODE RB_RULE selects by the routing rule `spec` instead (route_warp), and
+// RB_LOGITS only writes the logits [n_tok][n_expert] to w.
+#define RB_SOFTMAX 0
+#define RB_RULE 1
+#define RB_LOGITS 2
 #define RB_TOK 8
 #define RB_TOK_SMALL 4
 #define RB_SMALL_MAX 64   // batches up to this many tokens take TOK = 4
@@ -236,12 +241,13 @@ __device__ __forceinline__ float router_chain_dot(const float4 (&wv)[16], const 
 
 // grid RB_CL x ceil(n_tok / TOK) (cluster dims RB_CL); block NT;
 // dynamic shared memory: the cluster's token rows [TOK][2048].
-template <int TOK, int NT>
+template <int TOK, int NT, int MODE = RB_SOFTMAX>
 __global__ void __cluster_dims__(RB_CL, 1, 1) __launch_bounds__(NT)
     k_router_batch(const float *__restrict__ W, const float *__restrict__ x, int n_tok,
                    int n_expert, int k, int32_t *__restrict__ ids, float *__restrict__ w,
                    const int32_t *__restrict__ table, int ns, float delta, int use_prior,
-                   SlotState st, int observe_layer_idx, const int32_t *__restrict__ pub) {
+                   SlotState st, int observe_layer_idx, const int32_t *__restrict__ pub,
+                   RouteSpec spec = RouteSpec{}) {
     namespace cg = cooperative_groups;
     static_assert(TOK % 2 == 0 && (TOK * 512) % NT == 0, "k_router_batch shape");
     extern __shared__ __align__(16) float xs[];          // [TOK][2048]
@@ -278,12 +284,19 @@ __global__ void __cluster_dims__(RB_CL, 1, 1) __launch_bounds__(NT)
             const int t2 = t + 1 < nt ? t + 1 : t;
             const float va = router_chain_dot(wr, xs + t * 2048, lane);
             const float vb = router_chain_dot(wr, xs + t2 * 2048, lane);
-            if (lane == 0) {
+            if (MODE == RB_LOGITS) {
+                if (lane == 0) {
+                    float *o = w + (size_t)(t0 + t) * n_expert + e0 + j;
+                    o[0] = va;
+                    if (t + 1 < nt) o[n_expert] = vb;
+                }
+            } else if (lane == 0) {
                 lg[t][j] = va;
                 if (t + 1 < nt) lg[t + 1][j] = vb;
             }
         }
     }
+    if (MODE == RB_LOGITS) return;
     cl.sync();   // every CTA's logits are in its shared memory
     if (r < nt && warp == 0) {
         for (int e = lane; e < n_expert; e += 32) {
@@ -296,7 +309,14 @@ __global__ void __cluster_dims__(RB_CL, 1, 1) __launch_bounds__(NT)
         int id_r = -1;
         float w_r = 0.0f;
         const bool pri = use_prior != 0;
-        switch (n_expert) {
+        if (MODE == RB_RULE) {
+            const int per_lane = (spec.per + spec.lanes - 1) / spec.lanes;   // <= 16 for 256 experts
+            if (per_lane <= 4) route_warp_row<4>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
+            else if (per_lane <= 8) route_warp_row<8>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
+            else route_warp_row<16>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
+            if (lane < k) sids[lane] = id_r;
+            __syncwarp();
+        } else switch (n_expert) {
             case 32: select_warp<1>(lgf, 1.0f, table, ns, delta, pri, k, lane, id_r, w_r, sids, sw, pub); break;
             case 64: select_warp<2>(lgf, 1.0f, table, ns, delta, pri, k, lane, id_r, w_r, sids, sw, pub); break;
             case 128: select_warp<4>(lgf, 1.0f, table, ns, delta, pri, k, lane, id_r, w_r, sids, sw, pub); break;
@@ -803,6 +823,44 @@ cudaError_t launch_router(const float *W, const float *x, int n_tok, int n_exper
                                           ids, w, logits, st ? *st : dummy,
                                           st ? observe_layer_idx : -1, pub);
     return cudaGetLastError();
+}
+
+template <int MODE>
+static cudaError_t router_batch_mode(const float *W, const float *x, int n_tok, int n_expert, int n_embd, int k,
+                                     int32_t *ids, float *w, const int32_t *table, int ns, float delta,
+                                     int use_prior, const SlotState *st, int observe_layer_idx,
+                                     const int32_t *pub, const RouteSpec &sp, cudaStream_t s) {
+    if (n_embd != 2048 || n_expert % RB_CL || n_expert > 256) return cudaErrorInvalidValue;
+    const bool small = n_tok <= RB_SMALL_MAX;
+    const int tok = small ? RB_TOK_SMALL : RB_TOK;
+    const size_t sm = sizeof(float) * (size_t)tok * 2048;
+    const void *fn = small ? (const void *)k_router_batch<RB_TOK_SMALL, 512, MODE>
+                           : (const void *)k_router_batch<RB_TOK, 256, MODE>;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    if (e != cudaSuccess) return e;
+    const int grid = (n_tok + tok - 1) / tok * RB_CL;
+    const SlotState sst = st ? *st : SlotState{};
+    const int obs = st ? observe_layer_idx : -1;
+    if (small)
+        k_router_batch<RB_TOK_SMALL, 512, MODE><<<grid, 512, sm, s>>>(W, x, n_tok, n_expert, k, ids, w, table, ns,
+                                                                      delta, use_prior, sst, obs, pub, sp);
+    else
+        k_router_batch<RB_TOK, 256, MODE><<<grid, 256, sm, s>>>(W, x, n_tok, n_expert, k, ids, w, table, ns, delta,
+                                                                use_prior, sst, obs, pub, sp);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_router_rule(const float *W, const float *x, int n_tok, int n_embd, const RouteSpec &sp,
+                               const int32_t *table, int ns, float delta, int use_prior, int32_t *ids, float *w,
+                               const SlotState *st, int observe_layer_idx, const int32_t *pub, cudaStream_t s) {
+    return router_batch_mode<RB_RULE>(W, x, n_tok, sp.n_expert, n_embd, sp.k, ids, w, table, ns, delta, use_prior,
+                                      st, observe_layer_idx, pub, sp, s);
+}
+
+cudaError_t launch_router_logits(const float *W, const float *x, int n_tok, int n_expert, int n_embd,
+                                 float *logits, cudaStream_t s) {
+    return router_batch_mode<RB_LOGITS>(W, x, n_tok, n_expert, n_embd, 0, nullptr, logits, nullptr, 0, 0.0f, 0,
+                                        nullptr, -1, nullptr, RouteSpec{}, s);
 }
 
 cudaError_t launch_experts(const ExpertSrc &src, const float *x, const int32_t *ids,

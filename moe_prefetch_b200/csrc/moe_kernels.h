@@ -6,8 +6,12 @@
 #include <cstdint>
 
 #include "moe_dev.cuh"
+#include "moe_route.cuh"
 
 namespace moe {
+
+// element types of the block operators (the MOE_DTYPE_* of include/moeb200.h)
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 
 // Where one layer's experts live: slot slabs on the device (slot stride =
 // per-expert bytes; table[e] == ns means not resident), the registered host
@@ -55,6 +59,14 @@ cudaError_t launch_router(const float *W, const float *x, int n_tok, int n_exper
                           const int32_t *table, int ns, float delta, int use_prior, int k,
                           int32_t *ids, float *w, float *logits, const SlotState *st,
                           int observe_layer_idx, const int32_t *pub, cudaStream_t s);
+// launch_router with a routing rule in place of softmax + top-k + renormalise
+// (n_embd 2048; prior and observation for single tokens only)
+cudaError_t launch_router_rule(const float *W, const float *x, int n_tok, int n_embd, const RouteSpec &sp,
+                               const int32_t *table, int ns, float delta, int use_prior, int32_t *ids, float *w,
+                               const SlotState *st, int observe_layer_idx, const int32_t *pub, cudaStream_t s);
+// the logits alone, [n_tok][n_expert], the same bits (n_embd 2048)
+cudaError_t launch_router_logits(const float *W, const float *x, int n_tok, int n_expert, int n_embd,
+                                 float *logits, cudaStream_t s);
 cudaError_t launch_experts(const ExpertSrc &src, const float *x, const int32_t *ids,
                            const float *w, int n_tok, int k, int n_embd, int n_ff, int down_type,
                            float *act, const float *resid, float *y, int *err, cudaStream_t s);
@@ -107,7 +119,8 @@ cudaError_t launch_group(const int32_t *ids, int P, int n_expert, int tile, cons
 // bytes of scratch launch_experts_grouped needs for P pairs
 size_t grouped_scratch_bytes(int P, int n_embd, int n_ff);
 // gate/up + down over the grouped pairs (`scratch`: Q8_1 token rows and
-// activations; ypair [P][n_embd]), then the combine into y.  n_embd 2048.
+// activations; ypair [P][n_embd]), then the combine into y (y null: the caller
+// combines ypair by g.pair_pos).  n_embd 2048.
 cudaError_t launch_experts_grouped(const ExpertSrc &src, const float *x, const GroupBufs &g,
                                    int n_tok, int k, int n_embd, int n_ff, int down_type,
                                    const float *w, void *scratch, float *ypair, const float *resid,
@@ -115,6 +128,53 @@ cudaError_t launch_experts_grouped(const ExpertSrc &src, const float *x, const G
 cudaError_t launch_combine(const float *ypair, const int32_t *pair_pos, const float *w, int n_tok,
                            int k, int n_embd, const float *resid, float *y, cudaStream_t s,
                            const FlagWait *wait = nullptr, int *err = nullptr);
+
+// ---- routing from logits (moe_route.cu) ------------------------------------
+
+// logits [n_tok] rows of stride ld; prior and observation as launch_router's
+// (single tokens only; st null: neither)
+cudaError_t launch_route(const RouteSpec &sp, const void *logits, int dtype, int64_t ld, int n_tok, int32_t *ids,
+                         float *w, const int32_t *table, int ns, float delta, int use_prior, const SlotState *st,
+                         int observe_layer_idx, const int32_t *pub, cudaStream_t s);
+
+// ---- the norms around a block (moe_norm.cu) ---------------------------------
+
+enum { NORM_GATE_NONE = 0, NORM_GATE_TOKEN = 1, NORM_GATE_CHANNEL = 2, NORM_GATE_FULL = 3 };
+constexpr int NORM_MAX_EMBD = 16384;   // 1024 threads of 16 values
+
+struct NormArgs {
+    int n_tok, n_embd;
+    const void *r;              // residual [n_tok] rows of stride ld_r
+    const void *y;              // block output rows (null: none), or the expert rows [n_rows]
+    const int32_t *pos;         // [n_tok][k]: combine rows of y (fp32) with w, or null
+    const float *w;             // [n_tok][k]
+    const float *add;           // fp32 [n_tok][n_embd] added to the combine, or null
+    const float *post, *pre;    // [n_embd] or null
+    const void *gate;           // by gate_kind: [n_tok] rows (one value or n_embd), or fp32 [n_embd]
+    void *r_out, *x;            // either may be null
+    int64_t ld_r, ld_y, ld_gate, ld_ro, ld_x;
+    int k, n_rows, gate_kind, sigmoid;
+    float scale, eps, offset;
+};
+// dt_r: type of r, r_out; dt_y: of y, x and a token or full gate
+cudaError_t launch_block_norm(const NormArgs &a, int dt_r, int dt_y, cudaStream_t s);
+
+// ---- low-rank adapters (moe_adapters.cu) --------------------------------------
+
+struct AdapterArgs {
+    int n_tok, n_in, n_out, n_adapters, rank;   // rank: rows of each A (a multiple of 8)
+    const void *a, *b;          // [n_adapters][rank][lda], [n_adapters][n_out][rank]
+    int64_t lda;                // a multiple of 8, >= n_in; columns from n_in on are zero
+    const float *scale;         // [n_adapters]
+    const int32_t *ranks;       // [n_adapters] ranks in use, or null
+    const int32_t *ids;         // [n_tok]; outside [0, n_adapters): no adapter
+    const void *x, *y;          // y null: zeros
+    void *out;                  // may be y
+    int64_t ld_x, ld_y, ld_out;
+};
+constexpr int ADAPTER_MAX_RANK = 128;
+constexpr int ADAPTER_MAX_IN = 16384;
+cudaError_t launch_adapters(const AdapterArgs &a, int dt_x, int dt_w, int dt_out, cudaStream_t s);
 
 // ---- expert-parallel dispatch (moe_ep.cu) ----------------------------------
 
@@ -149,7 +209,7 @@ cudaError_t launch_ep_push(const EpMail &m, uint8_t *const *peer, const int32_t 
 // fp16 elements of scratch the GEMM needs for P pairs (token tiles + activation tiles)
 size_t gemm_scratch_halves(int n_expert, int P, int n_embd, int n_ff);
 // gate/up + down on tcgen05 over pairs grouped with tile GM_NT, then the
-// combine.  Q6_K down only; n_embd and n_ff multiples of 128.
+// combine (y null: left to the caller).  Q6_K down only; n_embd and n_ff multiples of 128.
 cudaError_t launch_experts_gemm(const ExpertSrc &src, const float *x, const GroupBufs &g,
                                 int n_tok, int k, int n_embd, int n_ff, int down_type,
                                 const float *w, void *scratch, float *ypair, const float *resid,

@@ -311,6 +311,91 @@ class MoeStack:
                  "moe_layer_forward_noalloc")
         return y
 
+    def set_routing(self, layer, routing):
+        """Route `layer` by a Routing (n_expert experts, top n_used) in
+        layer_forward, layer_forward_path, layer_forward_noalloc, block_forward
+        and expert parallelism; None: softmax, top-k, renormalise.  decode
+        refuses a stack that has any."""
+        if routing is None:
+            self._ck(self.lib.moe_set_routing(self.ctx, layer, None, None), "moe_set_routing")
+            return
+        self._ck(self.lib.moe_set_routing(self.ctx, layer, C.byref(routing.cfg), _ptr(routing.bias)),
+                 "moe_set_routing")
+
+    def block_forward(self, layer, x, r=None, norm=None, gate=None, adapter_ids=None, router_adapters=None,
+                      adapters=None, out=None, path="auto", stream=None):
+        """One expert layer with what is around it.  x [n_tok, n_embd] fp32 is
+        the pre-norm's output.  router_adapters (AdapterSet n_embd ->
+        n_expert) add to the router's logits and adapters (n_embd -> n_embd)
+        to the layer's output, chosen by adapter_ids int32 [n_tok].
+
+        With norm (a BlockNorm) the combine, the post norm, the gate, the
+        residual r and the next block's pre-norm are one kernel; returns (r',
+        x', ids, w), x' None when the norm has no second one.  out: the (r', x')
+        to write (r' may be r, x' may be x).  Without norm returns (y, ids, w)."""
+        if stream is not None:
+            from .block import _on_stream
+            sets = [t for s in (router_adapters, adapters) if s is not None for t in (s.a, s.b, s.scale, s.rank)]
+            return _on_stream(lambda: self.block_forward(layer, x, r, norm, gate, adapter_ids, router_adapters,
+                                                         adapters, out, path), stream,
+                              [x, r, gate, adapter_ids] + sets + ([norm.post, norm.pre] if norm else []) +
+                              list(out or ()))
+        self.start()
+        shape = (x.shape[0], self.n_embd)
+        n_tok = x.shape[0]
+        named = {"x": x, "r": r}
+        if out is not None:
+            named.update({"out r'": out[0], "out x'": out[1]})
+        for name, t in named.items():
+            if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous()
+                                  or t.device != self.device):
+                raise ValueError(f"{name} must be a contiguous fp32 {list(shape)} on {self.device}")
+        for s, n_out in ((router_adapters, self.n_expert), (adapters, self.n_embd)):
+            if s is None:
+                continue
+            if s.device != self.device or (s.n_in, s.n_out) != (self.n_embd, n_out):
+                raise ValueError(f"adapters of {s.n_in} -> {s.n_out} on {s.device}, expected {self.n_embd} -> "
+                                 f"{n_out} on {self.device}")
+            if adapter_ids is None:
+                raise ValueError("adapters need adapter_ids")
+            s.check_ids(adapter_ids, n_tok)
+        if (norm is None) != (r is None) or (norm is None and (gate is not None or out is not None)):
+            raise ValueError("a norm and the residual r come together; gate and out need them")
+        blk = _lib.MoeBlock()
+        if router_adapters is not None:
+            blk.router_adapters = C.pointer(router_adapters.st)
+        if adapters is not None:
+            blk.adapters = C.pointer(adapters.st)
+        if adapter_ids is not None:
+            blk.adapter_ids = adapter_ids.data_ptr()
+        slots = {layer: self.tables(layer)["expert_slot"]} if self._trace is not None else None
+        y = r_out = x_out = None
+        if norm is None:
+            y = torch.empty_like(x)
+        else:
+            if norm.n_embd != self.n_embd:
+                raise ValueError(f"a norm of {norm.n_embd} beside n_embd {self.n_embd}")
+            for t in (norm.post, norm.pre):
+                if t is not None and t.device != self.device:
+                    raise ValueError(f"the norm's weights are on {t.device}, expected {self.device}")
+            if out is not None and ((out[1] is not None) != norm.with_x or out[0] is None and out[1] is None):
+                raise ValueError("out must be (r', x'), with None for x' without a second norm")
+            r_out, x_out = out if out is not None else (torch.empty_like(r),
+                                                        torch.empty_like(x) if norm.with_x else None)
+            blk.norm = C.pointer(norm.with_gate(gate, n_tok, torch.float32, self.device))
+            blk.r, blk.r_out = r.data_ptr(), None if r_out is None else r_out.data_ptr()
+            blk.x_out = None if x_out is None else x_out.data_ptr()
+        ids = torch.empty(n_tok, self.n_used, dtype=torch.int32, device=x.device)
+        w = torch.empty(n_tok, self.n_used, dtype=torch.float32, device=x.device)
+        with torch.cuda.device(self.device):
+            rc = self.lib.moe_block_forward(self.ctx, layer, _ptr(x), n_tok, C.byref(blk), _ptr(y), _ptr(ids),
+                                            _ptr(w), {"auto": 0, "gemv": 1, "gemm": 2}[path],
+                                            _stream(torch.cuda.current_stream(self.device)))
+        self._ck(rc, "moe_block_forward")
+        if slots is not None and n_tok:
+            self._trace_routes({layer: ids.cpu().numpy()}, slots)
+        return (y, ids, w) if norm is None else (r_out, x_out, ids, w)
+
     def decode(self, h, out=None, debug=False, stream=None, profile=False, starve=0, spec=0):
         """Batch-1 decode of h [n_tok, n_embd] (device) through every layer,
         one token after another; returns out (and the per-layer dumps when

@@ -610,7 +610,7 @@ int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const flo
  * n_in on zero); B = b + i * n_out * rank, n_out rows of rank.  rank is a
  * multiple of 8, <= 128; ranks[i] <= rank is how much of adapter i is used (what
  * lies beyond is never used; NULL: all).  a and b are 16-byte aligned.
- * n_in <= 16384.  ggml applies adapters beside a projection in build_lora_mm,
+ * n_in <= 16384, n_adapters <= 2047.  ggml applies adapters beside a projection in build_lora_mm,
  * which build_moe_ffn calls for the router (context of patches/0007:101-128);
  * there all tokens share them. */
 typedef struct moe_adapters {

@@ -24,23 +24,29 @@ ACTS = {"none": 0, "sigmoid": 1}
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
 
 
+# The current stream's handle without a Stream object (torch.cuda.current_stream
+# takes 2 us of a call's 9), where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _rows(t, name, width, dtypes=DTYPES):
     """Check a [n, width] device tensor with contiguous rows; its row stride."""
-    if t.dim() != 2 or t.shape[1] != width:
-        raise ValueError(f"{name} must be [n, {width}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise ValueError(f"{name} must be [n, {width}], got {tuple(shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} has type {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
-    if t.shape[0] <= 1:
-        if width > 1 and t.stride(1) != 1:
-            raise ValueError(f"{name}: the elements of a row must be contiguous")
-        return width
-    if width > 1 and t.stride(1) != 1:
+    ld, inner = t.stride()
+    if inner != 1 and width > 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
-    if t.stride(0) < width:
-        raise ValueError(f"{name}: rows overlap (row stride {t.stride(0)})")
-    return t.stride(0)
+    if shape[0] <= 1:
+        return width
+    if ld < width:
+        raise ValueError(f"{name}: rows overlap (row stride {ld})")
+    return ld
 
 
 def _vector(t, name, n, dtype, device):
@@ -67,19 +73,9 @@ def _on_stream(call, stream, tensors):
     return out
 
 
-class _Guard:
-    """The tensors' device made current for a launch, where it is not."""
-
-    def __init__(self, device):
-        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
+def _elsewhere(index):
+    """True when the tensors' device is not the current one."""
+    return index != torch.cuda.current_device()
 
 
 class Routing:
@@ -104,30 +100,34 @@ class Routing:
         if bias is not None and (bias.shape != (n_expert,) or bias.dtype != torch.float32):
             raise ValueError(f"bias must be fp32 [{n_expert}], got {bias.dtype} {tuple(bias.shape)}")
         self.bias = None if bias is None else bias.contiguous()
+        self.bias_ptr = None if bias is None else self.bias.data_ptr()
+        self.cfg_ref = C.byref(self.cfg)
 
     def __call__(self, logits, out=None, stream=None):
         """logits [n, n_expert] (fp32, bf16 or fp16) -> (ids, w); out: the
         (ids, w) to write."""
         if stream is not None:
             return _on_stream(lambda: self(logits, out), stream, (logits, self.bias) + (out or ()))
+        index = logits.get_device()
+        if index >= 0 and _elsewhere(index):
+            with torch.cuda.device(index):
+                return self(logits, out)
         ld = _rows(logits, "logits", self.n_expert)
-        device, n = logits.device, logits.shape[0]
+        device, n, k = logits.device, logits.shape[0], self.k
         bias = self.bias
         if bias is not None and bias.device != device:
             raise ValueError(f"the bias is on {bias.device}, the logits are on {device}")
-        with _Guard(device):
-            if out is None:
-                ids = torch.empty(n, self.k, dtype=torch.int32, device=device)
-                w = torch.empty(n, self.k, dtype=torch.float32, device=device)
-            else:
-                ids, w = out
-                if (ids.shape != (n, self.k) or w.shape != (n, self.k) or ids.dtype != torch.int32
-                        or w.dtype != torch.float32 or not ids.is_contiguous() or not w.is_contiguous()):
-                    raise ValueError(f"out must be contiguous int32 and fp32 [{n}, {self.k}]")
-                _same_device(device, ids=ids, w=w)
-            rc = self.lib.moe_route(C.byref(self.cfg), logits.data_ptr(), DTYPES[logits.dtype], ld, n,
-                                    None if bias is None else bias.data_ptr(), ids.data_ptr(), w.data_ptr(),
-                                    torch.cuda.current_stream(device).cuda_stream)
+        if out is None:
+            ids = torch.empty(n, k, dtype=torch.int32, device=device)
+            w = torch.empty(n, k, dtype=torch.float32, device=device)
+        else:
+            ids, w = out
+            if (ids.shape != (n, k) or w.shape != (n, k) or ids.dtype != torch.int32 or w.dtype != torch.float32
+                    or not ids.is_contiguous() or not w.is_contiguous()):
+                raise ValueError(f"out must be contiguous int32 and fp32 [{n}, {k}]")
+            _same_device(device, ids=ids, w=w)
+        rc = self.lib.moe_route(self.cfg_ref, logits.data_ptr(), DTYPES[logits.dtype], ld, n, self.bias_ptr,
+                                ids.data_ptr(), w.data_ptr(), _raw_stream(index))
         if rc:
             check(rc, None, "moe_route")
         return ids, w
@@ -157,8 +157,14 @@ class BlockNorm:
         self.nm = MoeNorm(n_embd, GATE_NONE, ACTS[gate_act], scale, eps, weight_offset,
                           None if self.post is None else self.post.data_ptr(),
                           None if self.pre is None else self.pre.data_ptr(), None, 0)
-        check(self.lib.moe_block_norm(C.byref(self.nm), None, 0, n_embd, None, 0, n_embd, None, n_embd, None, n_embd,
+        self.nm_ref = C.byref(self.nm)
+        check(self.lib.moe_block_norm(self.nm_ref, None, 0, n_embd, None, 0, n_embd, None, n_embd, None, n_embd,
                                       0, None), None, "moe_block_norm")
+
+    def _weights_on(self, device):
+        for t in (self.post, self.pre):
+            if t is not None and t.device != device:
+                raise ValueError(f"the norm's weights are on {t.device}, expected {device}")
 
     def with_gate(self, gate, n, dtype, device):
         """The moe_norm of one call; gate None, [n, 1] (per row), [n_embd] (per
@@ -187,8 +193,9 @@ class BlockNorm:
     def _outputs(self, r, dtype, out):
         n, h = r.shape
         if out is None:
-            ro = torch.empty(n, h, dtype=r.dtype, device=r.device)
-            return ro, torch.empty(n, h, dtype=dtype, device=r.device) if self.with_x else None, h, h
+            device = r.device
+            ro = torch.empty(n, h, dtype=r.dtype, device=device)
+            return ro, torch.empty(n, h, dtype=dtype, device=device) if self.with_x else None, h, h
         ro, x = out
         if (x is not None) != self.with_x or ro is None and x is None:
             raise ValueError("out must be (r', x), with None for x without a second norm")
@@ -210,25 +217,28 @@ class BlockNorm:
         if stream is not None:
             return _on_stream(lambda: self(r, y, gate, out), stream,
                               (r, y, gate, self.post, self.pre) + (out or ()))
+        index = r.get_device()
+        if index >= 0 and _elsewhere(index):
+            with torch.cuda.device(index):
+                return self(r, y, gate, out)
         ld_r = _rows(r, "r", self.n_embd)
         device, n = r.device, r.shape[0]
-        dtype, ld_y = r.dtype, self.n_embd
+        dtype, ld_y, y_ptr = r.dtype, self.n_embd, None
         if y is not None:
             ld_y = _rows(y, "y", self.n_embd)
-            dtype = y.dtype
+            dtype, y_ptr = y.dtype, y.data_ptr()
             if y.shape[0] != n:
                 raise ValueError(f"y has {y.shape[0]} rows, r has {n}")
-        if out is not None and out[1] is not None and y is None:
+            if y.device != device:
+                raise ValueError(f"y is on {y.device}, expected {device}")
+        elif out is not None and out[1] is not None:
             dtype = out[1].dtype
-        _same_device(device, y=y, post=self.post, pre=self.pre)
-        nm = self.with_gate(gate, n, dtype, device)
-        with _Guard(device):
-            ro, x, lro, ldx = self._outputs(r, dtype, out)
-            rc = self.lib.moe_block_norm(C.byref(nm), r.data_ptr(), DTYPES[r.dtype], ld_r,
-                                         None if y is None else y.data_ptr(), DTYPES[dtype], ld_y,
-                                         None if ro is None else ro.data_ptr(), lro,
-                                         None if x is None else x.data_ptr(), ldx, n,
-                                         torch.cuda.current_stream(device).cuda_stream)
+        nm = self.nm_ref if gate is None else C.byref(self.with_gate(gate, n, dtype, device))
+        self._weights_on(device)
+        ro, x, lro, ldx = self._outputs(r, dtype, out)
+        rc = self.lib.moe_block_norm(nm, r.data_ptr(), DTYPES[r.dtype], ld_r, y_ptr, DTYPES[dtype], ld_y,
+                                     None if ro is None else ro.data_ptr(), lro,
+                                     None if x is None else x.data_ptr(), ldx, n, _raw_stream(index))
         if rc:
             check(rc, None, "moe_block_norm")
         return ro, x
@@ -240,6 +250,10 @@ class BlockNorm:
         if stream is not None:
             return _on_stream(lambda: self.combine(r, y_rows, pos, w, add, gate, out), stream,
                               (r, y_rows, pos, w, add, gate, self.post, self.pre) + (out or ()))
+        index = r.get_device()
+        if index >= 0 and _elsewhere(index):
+            with torch.cuda.device(index):
+                return self.combine(r, y_rows, pos, w, add, gate, out)
         f32 = (torch.float32,)
         h = self.n_embd
         ld_r, ld_rows = _rows(r, "r", h, f32), _rows(y_rows, "y_rows", h, f32)
@@ -250,16 +264,14 @@ class BlockNorm:
             raise ValueError(f"pos and w must be contiguous int32 and fp32 [{n}, k]")
         if add is not None and (add.shape != (n, h) or add.dtype != torch.float32 or not add.is_contiguous()):
             raise ValueError(f"add must be a contiguous fp32 [{n}, {h}]")
-        _same_device(device, y_rows=y_rows, pos=pos, w=w, add=add, post=self.post, pre=self.pre)
-        nm = self.with_gate(gate, n, torch.float32, device)
-        with _Guard(device):
-            ro, x, lro, ldx = self._outputs(r, torch.float32, out)
-            rc = self.lib.moe_combine_norm(C.byref(nm), r.data_ptr(), ld_r, y_rows.data_ptr(), ld_rows,
-                                           y_rows.shape[0], pos.data_ptr(), w.data_ptr(), k,
-                                           None if add is None else add.data_ptr(),
-                                           None if ro is None else ro.data_ptr(), lro,
-                                           None if x is None else x.data_ptr(), ldx, n,
-                                           torch.cuda.current_stream(device).cuda_stream)
+        _same_device(device, y_rows=y_rows, pos=pos, w=w, add=add)
+        nm = self.nm_ref if gate is None else C.byref(self.with_gate(gate, n, torch.float32, device))
+        self._weights_on(device)
+        ro, x, lro, ldx = self._outputs(r, torch.float32, out)
+        rc = self.lib.moe_combine_norm(nm, r.data_ptr(), ld_r, y_rows.data_ptr(), ld_rows, y_rows.shape[0],
+                                       pos.data_ptr(), w.data_ptr(), k, None if add is None else add.data_ptr(),
+                                       None if ro is None else ro.data_ptr(), lro,
+                                       None if x is None else x.data_ptr(), ldx, n, _raw_stream(index))
         if rc:
             check(rc, None, "moe_combine_norm")
         return ro, x
@@ -315,7 +327,8 @@ class AdapterSet:
         self.st = MoeAdapters(self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(),
                               None if self.rank is None else self.rank.data_ptr(), self.n, r + pr, self.n_in,
                               self.n_out, DTYPES[self.dtype], self.n_in + pc)
-        check(self.lib.moe_adapters_apply(C.byref(self.st), None, None, self.st.dtype, self.n_in, None, 0, None,
+        self.st_ref, self.index = C.byref(self.st), self.a.get_device()
+        check(self.lib.moe_adapters_apply(self.st_ref, None, None, self.st.dtype, self.n_in, None, 0, None,
                                           self.st.dtype, self.n_out, 0, None), None, "moe_adapters_apply")
 
     def check_ids(self, ids, n):
@@ -329,29 +342,33 @@ class AdapterSet:
         if stream is not None:
             return _on_stream(lambda: self(x, ids, y, out, out_dtype), stream,
                               (x, ids, y, out, self.a, self.b, self.scale, self.rank))
+        index = self.index
+        if _elsewhere(index):
+            with torch.cuda.device(index):
+                return self(x, ids, y, out, out_dtype)
+        device = self.device
         ld_x = _rows(x, "x", self.n_in)
         n = x.shape[0]
-        _same_device(self.device, x=x, y=y, out=out)
-        _vector(ids, "ids", n, torch.int32, self.device)
+        if x.device != device:
+            raise ValueError(f"x is on {x.device}, expected {device}")
+        ids_ptr = _vector(ids, "ids", n, torch.int32, device)
         ld_y = ld_o = self.n_out
+        y_ptr = None
         if y is not None:
             ld_y = _rows(y, "y", self.n_out)
-            if y.shape[0] != n:
-                raise ValueError(f"y has {y.shape[0]} rows, x has {n}")
-        with _Guard(self.device):
-            if out is None:
-                out = torch.empty(n, self.n_out, dtype=y.dtype if y is not None else out_dtype or x.dtype,
-                                  device=self.device)
-            else:
-                ld_o = _rows(out, "out", self.n_out)
-                if out.shape[0] != n or (y is not None and out.dtype != y.dtype):
-                    raise ValueError("out must have x's rows and y's type")
-            if out.dtype not in DTYPES:
-                raise ValueError(f"out has type {out.dtype}")
-            rc = self.lib.moe_adapters_apply(C.byref(self.st), ids.data_ptr(), x.data_ptr(), DTYPES[x.dtype], ld_x,
-                                             None if y is None else y.data_ptr(), ld_y, out.data_ptr(),
-                                             DTYPES[out.dtype], ld_o, n,
-                                             torch.cuda.current_stream(self.device).cuda_stream)
+            y_ptr = y.data_ptr()
+            if y.shape[0] != n or y.device != device:
+                raise ValueError(f"y has {y.shape[0]} rows on {y.device}, expected {n} on {device}")
+        if out is None:
+            out = torch.empty(n, self.n_out, dtype=y.dtype if y is not None else out_dtype or x.dtype, device=device)
+        else:
+            ld_o = _rows(out, "out", self.n_out)
+            if out.shape[0] != n or out.device != device or (y is not None and out.dtype != y.dtype):
+                raise ValueError("out must have x's rows and device and y's type")
+        if out.dtype not in DTYPES:
+            raise ValueError(f"out has type {out.dtype}")
+        rc = self.lib.moe_adapters_apply(self.st_ref, ids_ptr, x.data_ptr(), DTYPES[x.dtype], ld_x, y_ptr, ld_y,
+                                         out.data_ptr(), DTYPES[out.dtype], ld_o, n, _raw_stream(index))
         if rc:
             check(rc, None, "moe_adapters_apply")
         return out

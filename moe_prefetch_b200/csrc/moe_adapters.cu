@@ -2,122 +2,690 @@
 //
 //   out[t] = y[t] + scale[a] * B[a] (A[a] x[t]),   a = ids[t]
 //
-// with A [rank][n_in] and B [n_out][rank] in 16 bits.  The low-rank vector
-// A x stays in fp32 between the two products.
+// with A [rank][n_in] and B [n_out][rank] in 16 bits.
+//
+// k_adapters: a cluster of CTAs takes one tile of up to M tokens that use the
+// same adapter, wherever they stand in the batch (each CTA finds its tile's
+// tokens from the ids itself, so there is no grouping launch and no
+// workspace).  The cluster's CTAs split n_in for the first product, add their
+// partial A x through distributed shared memory, and split n_out for the
+// second.  The weights of an adapter are then read once per tile, x once, and
+// y and out once.
+//
+// The work is bound by memory (2 * rank flops per 16-bit weight and row) and
+// for few tokens by latency, so the products run on warp-level mma: a tcgen05
+// tile has at least 64 rows and a TMEM round trip, and decoded tokens fill a
+// few rows of one adapter.  16-bit x and all weights are exact operands.  An
+// fp32 x is split into two tf32 parts (22 bits).  A x stays in fp32 until the
+// second product, which splits it into parts of the weights' type: two for a
+// 16-bit output (bf16: 2^-18 of a term, against the output's 2^-9) and for fp16
+// weights (2^-24, each row scaled into fp16's range by a power of two), three
+// bf16 parts (2^-27) for an fp32 output.
 #include "moe_kernels.h"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <type_traits>
+
 namespace moe {
 
-__device__ __forceinline__ float ad_f32(float v) { return v; }
-__device__ __forceinline__ float ad_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float ad_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void ad_store(float *p, float v) { *p = v; }
-__device__ __forceinline__ void ad_store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16(v); }
-__device__ __forceinline__ void ad_store(__half *p, float v) { *p = __float2half(v); }
+namespace {
 
-// eight 16-bit weights at a 16-byte boundary
-__device__ __forceinline__ void ad_w8(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
+constexpr int AD_THREADS = 256;
+constexpr int AD_WARPS = AD_THREADS / 32;
+constexpr int AD_IDS = 16;            // ids per thread and pass of the search
+
+// columns of x per step of the first product: one k16 step per warp (M = 16), two per warp (M = 64)
+template <int M> constexpr int ad_kc() { return M == 16 ? 128 : 64; }
+// output columns per step of the second product: 2 (M = 16) or 4 (M = 64) mma tiles per warp
+template <int M> constexpr int ad_nc() { return M == 16 ? 128 : 64; }
+
+struct AdSmem {   // byte offsets in dynamic shared memory
+    int x_stage, a_stage, stages;   // the ring of the first product: stages * (x_stage + a_stage)
+    int b_stage, y_stage, b_stages, off_b;   // the ring of the second: b_stages * (b_stage + y_stage)
+    // over the first ring once it is done: partial sums of the warps, then the
+    // parts of A x (at 0); the CTA's partial A x (off_part)
+    int off_part;
+    int off_hist;                   // [n_adapters + 1]
+    int bytes;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {   // zero-fills to 16
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void ad_w8(const __half *p, float (&v)[8]) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // tf32
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-#define AD_THREADS 256
+// v = hi + lo: hi the leading 11 bits, lo the rest (of which tf32 keeps 11)
+__device__ __forceinline__ void split(float v, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(v) & 0xffffe000u;
+    lo = v == __uint_as_float(hi) ? 0u : __float_as_uint(v - __uint_as_float(hi));   // (inf - inf is no remainder)
+}
 
-// One CTA per token: x in shared memory, a warp per row of A, then a thread
-// per row of B.
-template <typename TX, typename TW, typename TO>
-__global__ void __launch_bounds__(AD_THREADS) k_adapter_row(AdapterArgs p) {
-    extern __shared__ __align__(16) float xs[];   // [lda]
-    __shared__ float low[ADAPTER_MAX_RANK];
-    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int a = p.ids[t];
-    const bool have = a >= 0 && a < p.n_adapters;
-    int rank = 0;
-    if (have) rank = p.ranks ? min(max(p.ranks[a], 0), p.rank) : p.rank;
-    if (rank > 0) {
-        const TX *x = (const TX *)p.x + (int64_t)t * p.ld_x;
-        for (int i = threadIdx.x; i < (int)p.lda; i += AD_THREADS) xs[i] = i < p.n_in ? ad_f32(x[i]) : 0.0f;
+// two 16-bit weights as exact tf32 operands
+__device__ __forceinline__ void pair32(uint32_t u, uint32_t &b0, uint32_t &b1, __nv_bfloat16) {
+    b0 = u << 16;
+    b1 = u & 0xffff0000u;
+}
+__device__ __forceinline__ void pair32(uint32_t u, uint32_t &b0, uint32_t &b1, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    b0 = __float_as_uint(f.x);
+    b1 = __float_as_uint(f.y);
+}
+
+
+__device__ __forceinline__ uint2 ad_pack(const float (&v)[4], __nv_bfloat16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+__device__ __forceinline__ uint2 ad_pack(const float (&v)[4], __half) {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+
+// two neighbouring outputs in shared memory: u += f * (v0, v1)
+__device__ __forceinline__ void ad_add2(float *u, float v0, float v1, float f, bool fresh) {
+    float2 y = make_float2(0.0f, 0.0f);
+    if (!fresh) y = *reinterpret_cast<const float2 *>(u);
+    *reinterpret_cast<float2 *>(u) = make_float2(fmaf(v0, f, y.x), fmaf(v1, f, y.y));
+}
+template <typename T>
+__device__ __forceinline__ void ad_add2(T *u, float v0, float v1, float f, bool fresh) {
+    uint32_t y0 = 0, y1 = 0;
+    if (!fresh) pair32(*reinterpret_cast<const uint32_t *>(u), y0, y1, T());
+    const float a = fmaf(v0, f, __uint_as_float(y0)), b = fmaf(v1, f, __uint_as_float(y1));
+    if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2 *>(u) = __floats2half2_rn(a, b);
+    else
+        *reinterpret_cast<__nv_bfloat162 *>(u) = __floats2bfloat162_rn(a, b);
+}
+
+// 16 bytes of a row of n elements from element i on: asynchronous where the
+// row is aligned (vec), else element by element; zeros from n on and for a
+// null row.
+template <typename T>
+__device__ __forceinline__ void row16(uint8_t *dst, const T *row, int i, int n, bool vec) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int have = row ? min(max(n - i, 0), E) : 0;
+    if (have == 0) {
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    if (vec) {
+        cp16(smem_u32(dst), row + i, have * (int)sizeof(T));
+        return;
+    }
+    __align__(16) T v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < have ? row[i + e] : T(0.0f);
+    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(v);
+}
+
+}  // namespace
+
+// The tile of cluster `b`: its adapter (n_adapters: none) and tokens.  The
+// tokens of an adapter keep their order and are cut into tiles of M.  False: no
+// such tile.  Every CTA of a cluster finds the same.
+template <int M>
+__device__ __forceinline__ bool ad_find_tile(const AdapterArgs &p, int b, int *hist, int *s_tok, int &a_out, int &cnt_out) {
+    __shared__ int s_wc[AD_WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int na = p.n_adapters, n = p.n_tok, buckets = na + (p.y == p.out ? 0 : 1);   // in place, rows without an adapter stay
+    const uint32_t below = (1u << lane) - 1;
+    auto bucket = [&](int t) {   // -1: no token
+        if (t >= n) return -1;
+        const int v = __ldg(p.ids + t);
+        return v >= 0 && v < na ? v : na;
+    };
+    if (n <= 32) {   // one token per lane, every warp alike: a tile is known by its first token
+        const int id = bucket(lane);
+        const uint32_t same = __match_any_sync(MOE_FULL, id);
+        const int rank = __popc(same & below);
+        const uint32_t heads = __ballot_sync(MOE_FULL, id >= 0 && id < buckets && rank % M == 0);
+        const uint32_t me = __ballot_sync(MOE_FULL, (heads >> lane & 1) && __popc(heads & below) == b);
+        if (!me) return false;
+        const int l = __ffs(me) - 1;
+        a_out = __shfl_sync(MOE_FULL, id, l);
+        const int r0 = __shfl_sync(MOE_FULL, rank, l);
+        cnt_out = min(M, __popc(__shfl_sync(MOE_FULL, same, l)) - r0);
+        if (warp == 0) {
+            if (id == a_out && rank >= r0 && rank < r0 + M) s_tok[rank - r0] = lane;
+            if (lane >= cnt_out && lane < M) s_tok[lane] = -1;
+        }
+        static_assert(M <= 64, "the entries past a short tile are cleared below");
+        if (M > 32 && warp == 1 && lane + 32 < M) s_tok[lane + 32] = -1;
         __syncthreads();
-        const float scale = p.scale[a];
-        for (int r = warp; r < p.rank; r += AD_THREADS / 32) {
-            float acc[8] = {};
-            if (r < rank) {
-                const TW *ar = (const TW *)p.a + ((int64_t)a * p.rank + r) * p.lda;
-                for (int i = 8 * lane; i < (int)p.lda; i += 256) {
-                    float w[8];
-                    ad_w8(ar + i, w);
+        return true;
+    }
+    // count the tokens of each adapter, then look for tile b.  A thread holds up
+    // to AD_IDS neighbouring ids, whose runs it counts with one addition each.
+    const int per = min(AD_IDS, (n + AD_THREADS - 1) / AD_THREADS), block = AD_THREADS * per;
+    int id[AD_IDS];
+    auto load = [&](int base) {
+        const int t0 = base + tid * per;
+        if (per == AD_IDS && ((uintptr_t)p.ids & 15) == 0 && base + block <= n) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) acc[c] = fmaf(w[c], xs[i + c], acc[c]);
+            for (int i = 0; i < AD_IDS; i += 4) {
+                const int4 v = __ldg(reinterpret_cast<const int4 *>(p.ids + t0 + i));
+                id[i] = v.x; id[i + 1] = v.y; id[i + 2] = v.z; id[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < AD_IDS; ++i)
+                if (i < per) id[i] = __ldg(p.ids + min(t0 + i, n - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < AD_IDS; ++i)
+            id[i] = i >= per || t0 + i >= n ? -1 : id[i] >= 0 && id[i] < na ? id[i] : na;
+    };
+    load(0);
+    for (int i = tid; i < na + 1; i += AD_THREADS) hist[i] = 0;
+    if (tid < M) s_tok[tid] = -1;
+    __syncthreads();
+    for (int base = 0; base < n; base += block) {
+        if (base) load(base);
+        int run = 1;
+#pragma unroll
+        for (int i = 0; i < AD_IDS; ++i) {
+            if (i >= per) break;
+            const int next = i + 1 < AD_IDS ? id[i + 1 < AD_IDS ? i + 1 : i] : -1;
+            if (i + 1 < per && next == id[i]) ++run;
+            else {
+                if (id[i] >= 0) atomicAdd(hist + id[i], run);
+                run = 1;
+            }
+        }
+    }
+    __syncthreads();
+    int a = -1, j0 = 0, before = 0;
+    for (int i0 = 0; i0 < buckets && a < 0; i0 += 32) {   // every warp alike
+        const int c = i0 + lane < buckets ? hist[i0 + lane] : 0;
+        const int tiles = (c + M - 1) / M;
+        int end = tiles;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(MOE_FULL, end, off);
+            if (lane >= off) end += o;
+        }
+        const uint32_t in = __ballot_sync(MOE_FULL, b < before + end);
+        if (in) {
+            const int l = __ffs(in) - 1;
+            a = i0 + l;
+            j0 = (b - before - (__shfl_sync(MOE_FULL, end, l) - __shfl_sync(MOE_FULL, tiles, l))) * M;
+            cnt_out = min(M, __shfl_sync(MOE_FULL, c, l) - j0);
+        }
+        before += __shfl_sync(MOE_FULL, end, 31);
+    }
+    if (a < 0) return false;
+    a_out = a;
+    // its tokens: those of rank [j0, j0 + M) among the adapter's
+    int run = 0;
+    for (int base = 0; base < n && run < j0 + M; base += block) {
+        if (n > block) load(base);
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < AD_IDS; ++i) mine += id[i] == a ? 1 : 0;
+        int pos = mine;   // inclusive prefix over the warp, then over the warps
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(MOE_FULL, pos, off);
+            if (lane >= off) pos += o;
+        }
+        if (lane == 31) s_wc[warp] = pos;
+        __syncthreads();
+        pos += run - mine - j0;
+#pragma unroll
+        for (int w = 0; w < AD_WARPS; ++w) {
+            const int c = s_wc[w];
+            if (w < warp) pos += c;
+            run += c;
+        }
+        if (mine && pos < M && pos + mine > 0) {
+            const int t0 = base + tid * per;
+#pragma unroll
+            for (int i = 0; i < AD_IDS; ++i)
+                if (id[i] == a) {
+                    if (pos >= 0 && pos < M) s_tok[pos] = t0 + i;
+                    ++pos;
+                }
+        }
+        __syncthreads();
+    }
+    return true;
+}
+
+// out rows of the tile = y rows (or zeros), columns [o0, o1): rows without an
+// adapter, or of an adapter of rank 0.
+template <typename TO>
+__device__ __forceinline__ void ad_copy_rows(const AdapterArgs &p, const int *s_tok, int cnt, int o0, int o1) {
+    for (int m = threadIdx.x >> 5; m < cnt; m += AD_WARPS) {
+        const int64_t t = s_tok[m];
+        const TO *y = (const TO *)p.y + t * p.ld_y;
+        TO *out = (TO *)p.out + t * p.ld_out;
+        for (int o = o0 + (int)(threadIdx.x & 31); o < o1; o += 32) out[o] = p.y ? y[o] : TO(0.0f);
+    }
+}
+
+// grid: tiles * cluster; M tokens per tile, up to 8 * NT ranks.  VEC: the rows of
+// x, y and out start at 16-byte boundaries.
+template <typename TX, typename TW, typename TO, int M, int NT, bool VEC>
+__global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(AdapterArgs p, AdSmem L) {
+    namespace cg = cooperative_groups;
+    constexpr bool X16 = sizeof(TX) == 2;
+    constexpr bool SCALED = std::is_same<TW, __half>::value;
+    constexpr int P = !SCALED && sizeof(TO) == 4 ? 3 : 2;        // parts of A x
+    constexpr int KC = ad_kc<M>(), NC = ad_nc<M>();
+    constexpr int MT = M / 16, KW = AD_WARPS / MT;   // warps: MT row tiles x KW shares of the k steps
+    constexpr int XP = KC * (int)sizeof(TX) + (X16 ? 16 : 32);   // row pitches in bytes, free of bank conflicts
+    constexpr int AP = KC * 2 + 16;
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ int s_tok[M];
+    __shared__ float s_fac[M];
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), cr = (int)cl.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int a, cnt;
+    if (!ad_find_tile<M>(p, blockIdx.x / C, reinterpret_cast<int *>(sm + L.off_hist), s_tok, a, cnt)) return;
+    const int oc = (p.n_out + NC - 1) / NC;                  // output steps, this CTA's [s0, s1)
+    const int s0 = (int)((int64_t)cr * oc / C), s1 = (int)((int64_t)(cr + 1) * oc / C);
+    int rank = 0;
+    if (a < p.n_adapters) rank = p.ranks ? min(max(p.ranks[a], 0), p.rank) : p.rank;
+    if (rank == 0) {
+        if (p.y != p.out) ad_copy_rows<TO>(p, s_tok, cnt, s0 * NC, min(s1 * NC, p.n_out));
+        return;
+    }
+    const int r8 = (rank + 7) & ~7, nt = r8 / 8;     // ranks computed by the first product
+    const int r16 = (rank + 15) & ~15;               // and read by the second: zeros from `rank` on
+    const TW *A = (const TW *)p.a + (int64_t)a * p.rank * p.lda;
+    const TW *B = (const TW *)p.b + (int64_t)a * p.n_out * p.rank;
+    const int bp = ((p.rank + 15) & ~15) * 2 + 16;   // pitch of B and of the parts of A x
+
+    // ---- loads: chunk k of x and A for the first product, chunk o of B and y for the second.
+    // A thread always loads the same 16-byte columns of the same rows, a whole
+    // chunk without a test per element.
+    constexpr int XE = 16 / (int)sizeof(TX), XC = KC / XE, XR = AD_THREADS / XC, XN = M / XR;   // x: XN rows per thread
+    constexpr int AC = KC / 8, AR = AD_THREADS / AC, AN = (8 * NT + AR - 1) / AR;
+    static_assert(M % XR == 0, "whole passes over the rows of x");
+    const TX *xrow[XN];
+#pragma unroll
+    for (int j = 0; j < XN; ++j) {
+        const int t = s_tok[tid / XC + j * XR];
+        xrow[j] = t >= 0 ? (const TX *)p.x + (int64_t)t * p.ld_x : nullptr;
+    }
+    const uint32_t sm0 = smem_u32(sm);
+    auto load_k = [&](int k, int stage) {
+        const int xo = stage * (L.x_stage + L.a_stage) + tid / XC * XP + 16 * (tid % XC);
+        const int ao = stage * (L.x_stage + L.a_stage) + L.x_stage + tid / AC * AP + 16 * (tid % AC);
+        const int xc = k * KC + XE * (tid % XC), ac = k * KC + 8 * (tid % AC);
+        if (VEC && (k + 1) * KC <= p.n_in) {
+#pragma unroll
+            for (int j = 0; j < XN; ++j)
+                cp16(sm0 + xo + j * XR * XP, (xrow[j] ? xrow[j] : (const TX *)p.x) + xc, xrow[j] ? 16 : 0);
+#pragma unroll
+            for (int j = 0; j < AN; ++j) {
+                const int r = tid / AC + j * AR;
+                if (r < r8) cp16(sm0 + ao + j * AR * AP, A + (r < rank ? r * p.lda : 0) + ac, r < rank ? 16 : 0);
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < XN; ++j) row16<TX>(sm + xo + j * XR * XP, xrow[j], xc, p.n_in, VEC);
+#pragma unroll
+        for (int j = 0; j < AN; ++j) {
+            const int r = tid / AC + j * AR;
+            if (r < r8) row16<TW>(sm + ao + j * AR * AP, r < rank ? A + (int64_t)r * p.lda : nullptr, ac, (int)p.lda, true);
+        }
+    };
+    constexpr int BT = AD_THREADS / NC, BN = NT > BT ? NT / BT : 1;      // B: threads per row, 16-byte columns of each
+    constexpr int YP = NC * (int)sizeof(TO) + (sizeof(TO) == 4 ? 32 : 16);
+    constexpr int YE = 16 / (int)sizeof(TO), YC = NC / YE, YR = AD_THREADS / YC, YN = M / YR;   // y and out
+    static_assert(M % YR == 0, "whole passes over the rows of y");
+    int yt[YN];
+#pragma unroll
+    for (int j = 0; j < YN; ++j) yt[j] = s_tok[tid / YC + j * YR];
+    auto load_b = [&](int o, int stage) {
+        const int so = L.off_b + stage * (L.b_stage + L.y_stage);
+        const int bo = so + tid / BT * bp + 16 * (tid % BT), yo = so + L.b_stage + tid / YC * YP + 16 * (tid % YC);
+        const int row = o * NC + tid / BT, yc = o * NC + YE * (tid % YC);
+        const bool full = (o + 1) * NC <= p.n_out;
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+            const int c = tid % BT + j * BT;
+            if (8 * c >= r16) continue;
+            const TW *src = B + (int64_t)row * p.rank;
+            if (full && 8 * c + 8 <= rank) cp16(sm0 + bo + 16 * BT * j, src + 8 * c, 16);
+            else row16<TW>(sm + bo + 16 * BT * j, row < p.n_out ? src : nullptr, 8 * c, rank, true);
+        }
+        if (!p.y) return;
+#pragma unroll
+        for (int j = 0; j < YN; ++j) {
+            if (yt[j] < 0) continue;
+            const TO *src = (const TO *)p.y + (int64_t)yt[j] * p.ld_y;
+            if (VEC && full) cp16(sm0 + yo + j * YR * YP, src + yc, 16);
+            else row16<TO>(sm + yo + j * YR * YP, src, yc, p.n_out, VEC);
+        }
+    };
+
+    // y's tile comes into L2 while the first product runs
+    if (p.y) {
+        constexpr int LE = 128 / (int)sizeof(TO);
+        const int c0 = s0 * NC, lines = (min(s1 * NC, p.n_out) - c0 + LE - 1) / LE;
+        for (int i = warp; i < cnt; i += AD_WARPS)
+            for (int l = lane; l < lines; l += 32)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"((const TO *)p.y + (int64_t)s_tok[i] * p.ld_y + c0 + l * LE));
+    }
+    // ---- first product: this CTA's share of n_in, one MT x KW grid of warps
+    const int kc = ((int)p.lda + KC - 1) / KC;
+    const int k0 = (int)((int64_t)cr * kc / C), k1 = (int)((int64_t)(cr + 1) * kc / C);
+    const int mt = warp % MT, kw = warp / MT;
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+    for (int s = 0; s < L.stages - 1; ++s) {
+        if (k0 + s < k1) load_k(k0 + s, s);
+        cp_commit();
+    }
+    int stage = 0;
+    for (int k = k0; k < k1; ++k) {
+        if (L.stages == 3) cp_wait<1>();
+        else cp_wait<0>();
+        __syncthreads();
+        if (k + L.stages - 1 < k1) load_k(k + L.stages - 1, stage == 0 ? L.stages - 1 : stage - 1);
+        cp_commit();
+        const uint8_t *xs = sm + stage * (L.x_stage + L.a_stage), *as = xs + L.x_stage;
+        stage = stage + 1 == L.stages ? 0 : stage + 1;
+#pragma unroll
+        for (int kk = kw; kk < KC / 16; kk += KW) {
+            if constexpr (X16) {
+                uint32_t af[4];
+                ldm4(af, smem_u32(xs + (16 * mt + (lane & 15)) * XP + 32 * kk + 16 * (lane >> 4)));
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    if (n >= nt) break;
+                    // rows of two n tiles (the last row again where the second lies past r8)
+                    const int r = min(8 * n + (lane & 7) + 8 * (lane >> 4), r8 - 1);
+                    uint32_t bf[4];
+                    ldm4(bf, smem_u32(as + r * AP + 32 * kk + 16 * (lane >> 3 & 1)));
+                    mma16(acc[n], af, bf[0], bf[1], TW());
+                    if (n + 1 < nt) mma16(acc[n + 1], af, bf[2], bf[3], TW());
+                }
+            } else {
+                // two k8 steps; the mma's k slots q, q + 4 hold columns 2q, 2q + 1 of both operands
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = 16 * kk + 8 * h + 2 * (lane & 3);
+                    const float2 u = *reinterpret_cast<const float2 *>(xs + (16 * mt + (lane >> 2)) * XP + 4 * col);
+                    const float2 v = *reinterpret_cast<const float2 *>(xs + (16 * mt + 8 + (lane >> 2)) * XP + 4 * col);
+                    uint32_t hi[4], lo[4];
+                    split(u.x, hi[0], lo[0]);
+                    split(v.x, hi[1], lo[1]);
+                    split(u.y, hi[2], lo[2]);
+                    split(v.y, hi[3], lo[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if (n >= nt) break;
+                        uint32_t b0, b1;
+                        pair32(*reinterpret_cast<const uint32_t *>(as + (8 * n + (lane >> 2)) * AP + 2 * col), b0, b1, TW());
+                        mma8(acc[n], lo, b0, b1);
+                        mma8(acc[n], hi, b0, b1);
+                    }
                 }
             }
-            const float v = warp_sum(((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7])));
-            if (lane == 0) low[r] = v * scale;
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();   // the ring is free
+
+    // the first chunks of B travel while the partial sums meet
+    for (int s = 0; s < L.b_stages - 1; ++s) {
+        if (s0 + s < s1) load_b(s0 + s, s);
+        cp_commit();
+    }
+    // ---- add the KW partial sums of the CTA, then those of the cluster, in order
+    {
+        const int pitch = p.rank + 8;
+        float *red = reinterpret_cast<float *>(sm);   // [KW][M][pitch]
+        float *mine = red + (kw * M + 16 * mt + (lane >> 2)) * pitch + 2 * (lane & 3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n >= nt) break;
+            *reinterpret_cast<float2 *>(mine + 8 * n) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2 *>(mine + 8 * pitch + 8 * n) = make_float2(acc[n][2], acc[n][3]);
         }
         __syncthreads();
-    }
-    const TO *y = (const TO *)p.y + (int64_t)t * p.ld_y;
-    TO *out = (TO *)p.out + (int64_t)t * p.ld_out;
-    for (int o = threadIdx.x; o < p.n_out; o += AD_THREADS) {
-        float acc = 0.0f;
-        if (rank > 0) {
-            const TW *br = (const TW *)p.b + ((int64_t)a * p.n_out + o) * p.rank;
-            for (int r = 0; r < rank; r += 8) {
-                float w[8];
-                ad_w8(br + r, w);
+        float *part = reinterpret_cast<float *>(sm + L.off_part);
+        {
+            constexpr int TR = AD_THREADS / M;         // threads per row, four columns each in turn
+            const int m = tid / TR;
+            for (int r = 4 * (tid % TR); r < r8; r += 4 * TR) {
+                const int at = m * pitch + r;
+                float4 v = *reinterpret_cast<const float4 *>(red + at);
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (r + c < rank) acc = fmaf(w[c], low[r + c], acc);
+                for (int w = 1; w < KW; ++w) {
+                    const float4 u = *reinterpret_cast<const float4 *>(red + w * M * pitch + at);
+                    v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+                }
+                *reinterpret_cast<float4 *>(part + at) = v;
             }
         }
-        ad_store(out + o, p.y ? ad_f32(y[o]) + acc : acc);
+        cl.sync();
+        // CTA cr adds up its M / C rows and gives the parts to the whole cluster
+        const float scale = p.scale[a];
+        const int rows = M / C, tr = min(32, AD_THREADS / rows);   // threads per row: a power of two
+        const int q = tid & (tr - 1), mr = tid / tr, m = cr * rows + mr;
+        if (mr < rows) {   // (whole warps: 32 * C / M rows of them)
+            constexpr int RT = 8 * NT / 4 * M / AD_THREADS > 0 ? 8 * NT / 4 * M / AD_THREADS : 1;   // groups of four per thread
+            float low[RT][4];
+            float top = 0.0f;                                   // the largest finite |low| of the row
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const int r = 4 * (q + j * tr);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) low[j][e] = 0.0f;
+                if (r >= r8) continue;
+                float4 u[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < C) u[c] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(part, c) + m * pitch + r);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < C) { low[j][0] += u[c].x; low[j][1] += u[c].y; low[j][2] += u[c].z; low[j][3] += u[c].w; }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    low[j][e] = r + e < rank ? low[j][e] * scale : 0.0f;
+                    if (SCALED && fabsf(low[j][e]) < INFINITY) top = fmaxf(top, fabsf(low[j][e]));
+                }
+            }
+            float up = 1.0f;
+            if (SCALED) {
+                for (int off = tr / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(MOE_FULL, top, off));
+                // 2^e brings the largest into [2^14, 2^15); e within the exponents whose inverse is normal too
+                const int e = top > 0.0f ? min(max(14 - ilogbf(top), -126), 126) : 0;
+                up = __int_as_float((127 + e) << 23);
+                if (q == 0)
+                    for (int c = 0; c < C; ++c) cl.map_shared_rank(s_fac, c)[m] = __int_as_float((127 - e) << 23);
+            }
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const int r = 4 * (q + j * tr);
+                if (r >= r16) continue;
+                uint2 w[P];
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = low[j][e] * up;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    w[i] = ad_pack(v, TW());
+                    float h[4];
+                    uint32_t b0, b1;
+                    pair32(w[i].x, b0, b1, TW());
+                    h[0] = __uint_as_float(b0); h[1] = __uint_as_float(b1);
+                    pair32(w[i].y, b0, b1, TW());
+                    h[2] = __uint_as_float(b0); h[3] = __uint_as_float(b1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = v[e] == h[e] ? 0.0f : v[e] - h[e];   // (inf - inf is no remainder)
+                }
+                for (int c = 0; c < C; ++c) {
+                    uint8_t *dst = cl.map_shared_rank(sm, c) + m * bp + 2 * r;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) *reinterpret_cast<uint2 *>(dst + i * M * bp) = w[i];
+                }
+            }
+        }
+        cl.sync();   // every CTA has all parts
     }
+
+    // ---- second product: [M][rank] x [rank][NC] per step; warps MT x KW over the n tiles.  The
+    // products are added to y's tile in shared memory, which is then written out in whole rows.
+    constexpr int WN = NC / 8 / KW;   // n tiles per warp
+    const int m_lo = 16 * mt + (lane >> 2);
+    const float f_lo = SCALED ? s_fac[m_lo] : 1.0f, f_hi = SCALED ? s_fac[m_lo + 8] : 1.0f;
+    const uint32_t a_off = sm0 + (16 * mt + (lane & 15)) * bp + 16 * (lane >> 4);
+    const uint32_t b_off = (8 * WN * kw + (lane & 7) + 8 * (lane >> 4)) * bp + 16 * (lane >> 3 & 1);
+    stage = 0;
+    for (int o = s0; o < s1; ++o) {
+        if (L.b_stages == 3) cp_wait<1>();
+        else cp_wait<0>();
+        __syncthreads();   // chunk o is there, and the chunk before is used up
+        if (o + L.b_stages - 1 < s1) load_b(o + L.b_stages - 1, stage == 0 ? L.b_stages - 1 : stage - 1);
+        cp_commit();
+        const int so = L.off_b + stage * (L.b_stage + L.y_stage);
+        stage = stage + 1 == L.b_stages ? 0 : stage + 1;
+        float d[WN][4];
+#pragma unroll
+        for (int n = 0; n < WN; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+#pragma unroll 2
+        for (int kk = 0; kk < r16 / 16; ++kk) {
+            uint32_t bf[WN / 2][4];
+#pragma unroll
+            for (int n = 0; n < WN; n += 2) ldm4(bf[n / 2], sm0 + so + b_off + 8 * n * bp + 32 * kk);
+#pragma unroll
+            for (int i = P - 1; i >= 0; --i) {   // the smallest parts first
+                uint32_t af[4];
+                ldm4(af, a_off + i * M * bp + 32 * kk);
+#pragma unroll
+                for (int n = 0; n < WN; ++n) mma16(d[n], af, bf[n / 2][2 * (n & 1)], bf[n / 2][2 * (n & 1) + 1], TW());
+            }
+        }
+        TO *ys = reinterpret_cast<TO *>(sm + so + L.b_stage + m_lo * YP) + 8 * WN * kw + 2 * (lane & 3);
+#pragma unroll
+        for (int n = 0; n < WN; ++n) {
+            ad_add2(ys + 8 * n, d[n][0], d[n][1], f_lo, !p.y);
+            ad_add2(ys + 8 * n + 8 * YP / (int)sizeof(TO), d[n][2], d[n][3], f_hi, !p.y);
+        }
+        __syncthreads();
+        const int yc = o * NC + YE * (tid % YC);
+        const uint8_t *yo = sm + so + L.b_stage + tid / YC * YP + 16 * (tid % YC);
+#pragma unroll
+        for (int j = 0; j < YN; ++j) {
+            if (yt[j] < 0 || yc >= p.n_out) continue;
+            TO *out = (TO *)p.out + (int64_t)yt[j] * p.ld_out + yc;
+            if (VEC && yc + YE <= p.n_out)
+                *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(yo + j * YR * YP);
+            else {
+                const TO *v = reinterpret_cast<const TO *>(yo + j * YR * YP);
+                for (int e = 0; e < YE && yc + e < p.n_out; ++e) out[e] = v[e];
+            }
+        }
+    }
+    cp_wait<0>();
+}
+
+template <typename TX, typename TW, typename TO, int M, int NT>
+static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
+    constexpr int KC = ad_kc<M>(), NC = ad_nc<M>();
+    constexpr int P = std::is_same<TW, __nv_bfloat16>::value && sizeof(TO) == 4 ? 3 : 2;
+    const int kc = (int)((p.lda + KC - 1) / KC), oc = (p.n_out + NC - 1) / NC;
+    // at most one partial tile per adapter in use (and for the rows without one)
+    const int64_t tiles = std::min<int64_t>(p.n_tok, ((int64_t)p.n_tok + M - 1) / M + std::min(p.n_adapters + 1, p.n_tok));
+    // CTAs per tile: enough to fill the GPU, at most one per step of a product
+    int C = 1;
+    while (C < 8 && tiles * C < 148 && 2 * C <= std::max(kc, oc)) C *= 2;
+    AdSmem L{};
+    L.x_stage = M * (KC * (int)sizeof(TX) + (sizeof(TX) == 2 ? 16 : 32));
+    L.a_stage = p.rank * (KC * 2 + 16);
+    const int pitch = p.rank + 8, KW = AD_WARPS / (M / 16), bp = ((p.rank + 15) & ~15) * 2 + 16;
+    const int red = KW * M * pitch * 4, low = P * M * bp, part = M * pitch * 4;
+    L.off_part = std::max(red, low);
+    L.b_stage = NC * bp;
+    L.y_stage = M * (NC * (int)sizeof(TO) + (sizeof(TO) == 4 ? 32 : 16));
+    // up to three stages each: as many as leave room for a second CTA on the SM, else two, else what fits
+    const int ks = std::max(2, std::min(3, kc / C + 1)), bs = std::max(2, std::min(3, oc / C + 1));
+    auto lay = [&](int k, int o, int limit) {
+        L.stages = k;
+        L.b_stages = o;
+        L.off_b = std::max(k * (L.x_stage + L.a_stage), L.off_part + part);
+        L.off_hist = L.off_b + o * (L.b_stage + L.y_stage);
+        L.bytes = L.off_hist + 4 * (p.n_adapters + 1);
+        return L.bytes <= limit;
+    };
+    constexpr int TWO = 111 * 1024, ONE = 226 * 1024;
+    if (!lay(ks, bs, TWO) && !lay(2, bs, TWO) && !lay(2, 2, TWO) && !lay(ks, bs, ONE) && !lay(2, 2, ONE))
+        return cudaErrorInvalidValue;
+    auto al = [](const void *q, int64_t ld, int size) {
+        return !q || (((uintptr_t)q | (uintptr_t)(ld * size)) & 15) == 0;
+    };
+    const bool vec = al(p.x, p.ld_x, (int)sizeof(TX)) && al(p.y, p.ld_y, (int)sizeof(TO)) &&
+                     al(p.out, p.ld_out, (int)sizeof(TO));
+    auto *kern = vec ? k_adapters<TX, TW, TO, M, NT, true> : k_adapters<TX, TW, TO, M, NT, false>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L.bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * C));
+    cfg.blockDim = dim3(AD_THREADS);
+    cfg.dynamicSmemBytes = L.bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = C;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, p, L);
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <typename TX, typename TW, typename TO>
 static cudaError_t adapters_go(const AdapterArgs &p, cudaStream_t s) {
-    const size_t smem = sizeof(float) * (size_t)p.lda;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(k_adapter_row<TX, TW, TO>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    k_adapter_row<TX, TW, TO><<<p.n_tok, AD_THREADS, smem, s>>>(p);
-    return cudaGetLastError();
+    // tiles of 16 rows until there are enough rows to fill larger ones
+    if (p.n_tok <= 512)
+        return p.rank <= 32 ? adapters_launch<TX, TW, TO, 16, 4>(p, s) : adapters_launch<TX, TW, TO, 16, 16>(p, s);
+    return p.rank <= 64 ? adapters_launch<TX, TW, TO, 64, 8>(p, s) : adapters_launch<TX, TW, TO, 64, 16>(p, s);
 }
 
 cudaError_t launch_adapters(const AdapterArgs &p, int dt_x, int dt_w, int dt_out, cudaStream_t s) {
-    if (p.n_tok == 0 || p.n_out == 0) return cudaSuccess;
-    if (dt_x == DT_F32 && dt_out == DT_F32) {
-        if (dt_w == DT_BF16) return adapters_go<float, __nv_bfloat16, float>(p, s);
-        if (dt_w == DT_F16) return adapters_go<float, __half, float>(p, s);
-    }
-    if (dt_x == DT_BF16 && dt_w == DT_BF16) {
-        if (dt_out == DT_BF16) return adapters_go<__nv_bfloat16, __nv_bfloat16, __nv_bfloat16>(p, s);
-        if (dt_out == DT_F32) return adapters_go<__nv_bfloat16, __nv_bfloat16, float>(p, s);
-    }
-    if (dt_x == DT_F16 && dt_w == DT_F16) {
-        if (dt_out == DT_F16) return adapters_go<__half, __half, __half>(p, s);
-        if (dt_out == DT_F32) return adapters_go<__half, __half, float>(p, s);
-    }
-    return cudaErrorInvalidValue;
+    if (p.n_tok == 0) return cudaSuccess;
+    if (dt_x == DT_F32 && dt_out == DT_F32)
+        return dt_w == DT_BF16 ? adapters_go<float, __nv_bfloat16, float>(p, s) : adapters_go<float, __half, float>(p, s);
+    if (dt_x != dt_w || (dt_out != dt_w && dt_out != DT_F32)) return cudaErrorInvalidValue;
+    if (dt_w == DT_BF16)
+        return dt_out == DT_F32 ? adapters_go<__nv_bfloat16, __nv_bfloat16, float>(p, s)
+                                : adapters_go<__nv_bfloat16, __nv_bfloat16, __nv_bfloat16>(p, s);
+    return dt_out == DT_F32 ? adapters_go<__half, __half, float>(p, s) : adapters_go<__half, __half, __half>(p, s);
 }
 
 }  // namespace moe

@@ -1865,6 +1865,7 @@ static const char *adapters_bad(const moe_adapters &s, int n_tok, int *code) {
     *code = MOE_ERR_UNSUPPORTED;
     if (s.rank > ADAPTER_MAX_RANK) return "rank is above 128";
     if (s.n_in > ADAPTER_MAX_IN) return "n_in is above 16384";
+    if (s.n_adapters > ADAPTER_MAX_SET) return "more than 2047 adapters";
     return nullptr;
 }
 

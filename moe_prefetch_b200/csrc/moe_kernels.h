@@ -174,6 +174,7 @@ struct AdapterArgs {
 };
 constexpr int ADAPTER_MAX_RANK = 128;
 constexpr int ADAPTER_MAX_IN = 16384;
+constexpr int ADAPTER_MAX_SET = 2047;   // adapters + 1 counters per CTA
 cudaError_t launch_adapters(const AdapterArgs &a, int dt_x, int dt_w, int dt_out, cudaStream_t s);
 
 // ---- expert-parallel dispatch (moe_ep.cu) ----------------------------------

@@ -415,6 +415,36 @@ def test_adapters_ragged_ranks_strides(n, xt, wt, ot):
     check_adapters(n, 256, 192, 5, 40, xt, wt, ot, order="one", with_y=False)
 
 
+@pytest.mark.parametrize("xt,wt,ot", TYPES)
+@pytest.mark.parametrize("n,n_in,n_out,na,r,order", [
+    (513, 192, 130, 3, 16, "mixed"), (700, 1000, 72, 4, 64, "sorted"), (1111, 136, 96, 9, 23, "sorted"),
+    (640, 256, 64, 2, 128, "mixed"), (4097, 64, 40, 50, 8, "mixed"), (8500, 32, 24, 2000, 8, "mixed")])
+def test_adapters_long(n, n_in, n_out, na, r, order, xt, wt, ot):
+    """Large tiles, several blocks of the token search, more adapters than fit one scan."""
+    check_adapters(n, n_in, n_out, na, r, xt, wt, ot, order=order, ragged=na < 10)
+
+
+@pytest.mark.parametrize("xt,wt,ot", TYPES)
+@pytest.mark.parametrize("n", [7, 600])
+def test_adapters_extreme_values(n, xt, wt, ot):
+    """An infinity or NaN stays in its row; rows of very different size keep
+    their own precision."""
+    from moe_prefetch_b200 import AdapterSet
+    a, b = (randn(2, 16, 128, seed=1) / 11).to(wt), (randn(2, 72, 16, seed=2) / 4).to(wt)
+    x = randn(n, 128, seed=3)
+    x[1] *= 2.0 ** -10
+    x[2] *= 2.0 ** 10
+    x[3, 5], x[4, 6], x[5] = math.inf, math.nan, 0.0
+    x = x.to(xt)
+    ids = torch.zeros(n, dtype=torch.int32).cuda()
+    scale = torch.tensor([0.5, 2.0]).cuda()
+    out = AdapterSet(a, b, scale=scale)(x, ids, out_dtype=ot)
+    rows = [t for t in range(n) if t not in (3, 4)]
+    want, bound = adapters_ref(x[rows], torch.zeros(len(rows), 72), a, b, scale, None, ids[rows])
+    close(out[rows], want, bound, "out")
+    assert not torch.isfinite(out[3]).any() and torch.isnan(out[4]).all()
+
+
 def test_adapters_lists_empty_refusals():
     from moe_prefetch_b200 import AdapterSet
     a = [randn(r, 96, seed=r).to(BF16) for r in (4, 9, 16)]

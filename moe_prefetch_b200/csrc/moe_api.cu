@@ -722,8 +722,8 @@ static cudaError_t route_tokens(moe_ctx *c, int layer, const float *x, int n_tok
     const int32_t *pub = cached ? c->st.slot_expert + c->slot_off[layer] : nullptr;
     if (logits) {
         const RouteSpec sp = m.ruled ? m.rule : route_spec(g.n_expert, g.n_used, 0, 1, 1, 1, 1, 1.0f, nullptr);
-        return launch_route(sp, logits, DT_F32, g.n_expert, n_tok, ids, w, table, m.ns, delta, prior, &c->st, obs,
-                            pub, s);
+        return one ? launch_route_one(sp, logits, ids, w, table, m.ns, delta, prior, c->st, layer, pub, s)
+                   : launch_route(sp, logits, DT_F32, g.n_expert, n_tok, ids, w, s);
     }
     if (m.ruled)
         return launch_router_rule(W, x, n_tok, g.n_embd, m.rule, table, m.ns, delta, prior, ids, w, &c->st, obs, pub,
@@ -1746,8 +1746,7 @@ extern "C" int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype
     if (!n_tok) return MOE_OK;
     CK(launch_route(route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
                                cfg->renorm, cfg->scale, bias),
-                    logits, dtype, ld, n_tok, ids, w, nullptr, 0, 0.0f, 0, nullptr, -1, nullptr,
-                    (cudaStream_t)stream));
+                    logits, dtype, ld, n_tok, ids, w, (cudaStream_t)stream));
     return MOE_OK;
 }
 

@@ -310,10 +310,8 @@ __global__ void __cluster_dims__(RB_CL, 1, 1) __launch_bounds__(NT)
         float w_r = 0.0f;
         const bool pri = use_prior != 0;
         if (MODE == RB_RULE) {
-            const int per_lane = (spec.per + spec.lanes - 1) / spec.lanes;   // <= 16 for 256 experts
-            if (per_lane <= 4) route_warp_row<4>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
-            else if (per_lane <= 8) route_warp_row<8>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
-            else route_warp_row<16>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
+            // 32, 64, 128 or 256 experts: at most 8 per lane, whatever the groups
+            route_warp_row<8>(lgf, spec, table, ns, delta, pri, pub, lane, id_r, w_r);
             if (lane < k) sids[lane] = id_r;
             __syncwarp();
         } else switch (n_expert) {
@@ -830,7 +828,8 @@ static cudaError_t router_batch_mode(const float *W, const float *x, int n_tok, 
                                      int32_t *ids, float *w, const int32_t *table, int ns, float delta,
                                      int use_prior, const SlotState *st, int observe_layer_idx,
                                      const int32_t *pub, const RouteSpec &sp, cudaStream_t s) {
-    if (n_embd != 2048 || n_expert % RB_CL || n_expert > 256) return cudaErrorInvalidValue;
+    if (n_embd != 2048 || n_expert % RB_CL || n_expert > 256 || (MODE == RB_RULE && route_per_lane(sp) > 8))
+        return cudaErrorInvalidValue;
     const bool small = n_tok <= RB_SMALL_MAX;
     const int tok = small ? RB_TOK_SMALL : RB_TOK;
     const size_t sm = sizeof(float) * (size_t)tok * 2048;

@@ -131,11 +131,13 @@ cudaError_t launch_combine(const float *ypair, const int32_t *pair_pos, const fl
 
 // ---- routing from logits (moe_route.cu) ------------------------------------
 
-// logits [n_tok] rows of stride ld; prior and observation as launch_router's
-// (single tokens only; st null: neither)
+// logits [n_tok] rows of stride ld, type dtype
 cudaError_t launch_route(const RouteSpec &sp, const void *logits, int dtype, int64_t ld, int n_tok, int32_t *ids,
-                         float *w, const int32_t *table, int ns, float delta, int use_prior, const SlotState *st,
-                         int observe_layer_idx, const int32_t *pub, cudaStream_t s);
+                         float *w, cudaStream_t s);
+// one token of a layer, with the prior and observation of launch_router
+cudaError_t launch_route_one(const RouteSpec &sp, const float *logits, int32_t *ids, float *w, const int32_t *table,
+                             int ns, float delta, int use_prior, const SlotState &st, int observe_layer_idx,
+                             const int32_t *pub, cudaStream_t s);
 
 // ---- the norms around a block (moe_norm.cu) ---------------------------------
 

@@ -91,48 +91,61 @@ __device__ __forceinline__ float norm_cta_sum(float v, float *part) {
 
 // One CTA per row; thread i holds the chunks of VEC values at VEC * (i + c *
 // blockDim.x), c < V.  SRC 0: y rows of type TY; 1: the combine of fp32 rows.
+// Everything the row needs is loaded before the first sum, so that one memory
+// latency covers it.
 template <typename TR, typename TY, int VEC, int V, int SRC>
 __global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
     __shared__ float part[2][32];
     const int t = blockIdx.x;
     const int H = a.n_embd;
     const float inv_h = 1.0f / (float)H;   // each square is scaled first: the sum overflows only where the mean does
-    float y[V][VEC], r[V][VEC];
+    float y[V][VEC], r[V][VEC], g[V][VEC], po[V][VEC];
     const TR *rr = (const TR *)a.r + (int64_t)t * a.ld_r;
+    float gt[1] = {0.0f};
+    if (a.gate_kind == NORM_GATE_TOKEN) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate, gt);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
         const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-        if (h < H) norm_load(rr + h, r[c]);
-        else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) r[c][i] = 0.0f;
-        }
+        for (int i = 0; i < VEC; ++i) y[c][i] = r[c][i] = po[c][i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) y[c][i] = 0.0f;
+        for (int i = 0; i < VEC; ++i) g[c][i] = 0.0f;
+        if (h >= H) continue;
+        norm_load(rr + h, r[c]);
+        if (SRC == 0 && a.y) norm_load((const TY *)a.y + (int64_t)t * a.ld_y + h, y[c]);
+        if (a.gate_kind == NORM_GATE_FULL) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate + h, g[c]);
+        else if (a.gate_kind == NORM_GATE_CHANNEL) norm_load((const float *)a.gate + h, g[c]);
+        if (a.post) norm_load(a.post + h, po[c]);
     }
-    if (SRC == 0) {
-        const TY *yr = (const TY *)a.y + (int64_t)t * a.ld_y;
-#pragma unroll
-        for (int c = 0; c < V; ++c) {
-            const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-            if (h < H && a.y) norm_load(yr + h, y[c]);
-        }
-    } else {
-        // the chain of k_combine: fma from 0 in rank order, then + add
+    if (SRC == 1) {
+        // the chain of k_combine: fma from 0 in rank order, then + add.  Four
+        // rows are in flight at a time.
         const float *rows = (const float *)a.y;
-        for (int j = 0; j < a.k; ++j) {
-            const int pos = a.pos[(int64_t)t * a.k + j];
-            const float w = a.w[(int64_t)t * a.k + j];
+        const int32_t *pos = a.pos + (int64_t)t * a.k;
+        const float *w = a.w + (int64_t)t * a.k;
+        constexpr int U = VEC * V <= 8 ? 4 : 2;
+        for (int j0 = 0; j0 < a.k; j0 += U) {
+            float v[U][V][VEC], wj[U];
 #pragma unroll
-            for (int c = 0; c < V; ++c) {
-                const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-                float v[VEC];
+            for (int u = 0; u < U; ++u) {
+                const int at = j0 + u < a.k ? pos[j0 + u] : -1;
+                wj[u] = j0 + u < a.k ? w[j0 + u] : 0.0f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
-                if (h < H && pos >= 0 && pos < a.n_rows) norm_load(rows + (int64_t)pos * a.ld_y + h, v);
+                for (int c = 0; c < V; ++c) {
+                    const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) y[c][i] = __fmaf_rn(w, v[i], y[c][i]);
+                    for (int i = 0; i < VEC; ++i) v[u][c][i] = 0.0f;
+                    if (h < H && at >= 0 && at < a.n_rows) norm_load(rows + (int64_t)at * a.ld_y + h, v[u][c]);
+                }
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u < a.k) {
+#pragma unroll
+                    for (int c = 0; c < V; ++c)
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) y[c][i] = __fmaf_rn(wj[u], v[u][c][i], y[c][i]);
+                }
         }
         if (a.add) {
 #pragma unroll
@@ -155,33 +168,18 @@ __global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
             for (int i = 0; i < VEC; ++i) ss = fmaf(y[c][i] * inv_h, y[c][i], ss);
         const float inv = 1.0f / sqrtf(norm_cta_sum(ss, part[0]) + a.eps);
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-            const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-            if (h < H) {
-                float p[VEC];
-                norm_load(a.post + h, p);
+        for (int c = 0; c < V; ++c)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) y[c][i] *= inv * (p[i] + a.offset);
-            }
-        }
+            for (int i = 0; i < VEC; ++i) y[c][i] *= inv * (po[c][i] + a.offset);
     }
     if (a.gate_kind != NORM_GATE_NONE) {
-        float gt[1] = {0.0f};
-        if (a.gate_kind == NORM_GATE_TOKEN) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate, gt);
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-            const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-            if (h >= H) continue;
-            float g[VEC];
-            if (a.gate_kind == NORM_GATE_FULL) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate + h, g);
-            else if (a.gate_kind == NORM_GATE_CHANNEL) norm_load((const float *)a.gate + h, g);
-            else {
+        for (int c = 0; c < V; ++c)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) g[i] = gt[0];
+            for (int i = 0; i < VEC; ++i) {
+                const float v = a.gate_kind == NORM_GATE_TOKEN ? gt[0] : g[c][i];
+                y[c][i] *= a.sigmoid ? 1.0f / (1.0f + expf(-v)) : v;
             }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) y[c][i] *= a.sigmoid ? 1.0f / (1.0f + expf(-g[i])) : g[i];
-        }
     }
     float ss = 0.0f;
     TR *ro = (TR *)a.r_out + (int64_t)t * a.ld_ro;
@@ -189,11 +187,11 @@ __global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
     for (int c = 0; c < V; ++c) {
         const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            r[c][i] = fmaf(a.scale, y[c][i], r[c][i]);
-            ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
-        }
+        for (int i = 0; i < VEC; ++i) r[c][i] = h < H ? fmaf(a.scale, y[c][i], r[c][i]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
         if (h < H && a.r_out) norm_store(ro + h, r[c]);
+        if (h < H && a.x && a.pre) norm_load(a.pre + h, po[c]);
     }
     if (!a.x) return;
     const float inv = 1.0f / sqrtf(norm_cta_sum(ss, part[1]) + a.eps);
@@ -201,13 +199,9 @@ __global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
 #pragma unroll
     for (int c = 0; c < V; ++c) {
         const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-        if (h < H) {
-            float p[VEC];
-            if (a.pre) norm_load(a.pre + h, p);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) p[i] = r[c][i] * inv * (a.pre ? p[i] + a.offset : 1.0f);
-            norm_store(xo + h, p);
-        }
+        for (int i = 0; i < VEC; ++i) r[c][i] *= inv * (a.pre ? po[c][i] + a.offset : 1.0f);
+        if (h < H) norm_store(xo + h, r[c]);
     }
 }
 

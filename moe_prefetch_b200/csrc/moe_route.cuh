@@ -22,7 +22,7 @@ namespace moe {
 struct RouteSpec {
     int n_expert, k, sigmoid, n_group, topk_group, group_top, renorm;
     int per;       // experts per group
-    int lanes;     // lanes per group: the largest power of two <= 32 / n_group
+    int log_lanes; // 2^log_lanes lanes per group: the largest power of two <= 32 / n_group
     float scale;
     const float *bias;   // [n_expert] or null
 };
@@ -34,36 +34,47 @@ constexpr int ROUTE_MAX_K = 32;
 // The rule of checked arguments, with its derived fields.
 inline RouteSpec route_spec(int n_expert, int k, int sigmoid, int n_group, int topk_group, int group_top, int renorm,
                             float scale, const float *bias) {
-    RouteSpec s{n_expert, k, sigmoid, n_group, topk_group, group_top, renorm, n_expert / n_group, 32, scale, bias};
-    while (s.lanes * n_group > 32) s.lanes >>= 1;
+    RouteSpec s{n_expert, k, sigmoid, n_group, topk_group, group_top, renorm, n_expert / n_group, 5, scale, bias};
+    while (n_group << s.log_lanes > 32) --s.log_lanes;
     return s;
 }
-// Experts each lane holds: per / lanes rounded up.  At most 30 for
-// ROUTE_MAX_EXPERT experts in up to ROUTE_MAX_GROUP groups (lanes * n_group
-// > 16).
-inline int route_per_lane(const RouteSpec &s) { return (s.per + s.lanes - 1) / s.lanes; }
+// Experts each lane holds.  At most 30 for ROUTE_MAX_EXPERT experts in up to
+// ROUTE_MAX_GROUP groups (more than 16 of the 32 lanes have a group).
+inline int route_per_lane(const RouteSpec &s) { return ((s.per - 1) >> s.log_lanes) + 1; }
 
-// The lane layout: group g's experts go to lanes [g * lanes, (g + 1) * lanes),
-// expert g * per + i + lanes * j to lane g * lanes + i as its j-th.  A group
-// score is then a butterfly over `lanes` lanes; with one group it is the plain
-// strided layout.  -1: the lane has no j-th expert.
-__device__ __forceinline__ int route_expert(const RouteSpec &s, int lane, int j) {
-    const int g = lane / s.lanes, i = (lane & (s.lanes - 1)) + s.lanes * j;
-    return g < s.n_group && i < s.per ? g * s.per + i : -1;
-}
+// The lane layout: with q = 2^log_lanes, group g's experts go to lanes [g q,
+// (g + 1) q), expert g * per + i + q j to lane g q + i as its j-th.  A group
+// score is then a butterfly over q lanes; with one group it is the plain strided
+// layout.
+struct RouteLane {
+    int group, first, step, count;   // experts first, first + step, ... (count of them)
+    __device__ __forceinline__ RouteLane(const RouteSpec &s, int lane) {
+        group = lane >> s.log_lanes;
+        step = 1 << s.log_lanes;
+        const int i = lane & (step - 1);
+        first = group * s.per + i;
+        count = group < s.n_group && i < s.per ? ((s.per - 1 - i) >> s.log_lanes) + 1 : 0;
+    }
+    __device__ __forceinline__ int expert(int j) const { return first + step * j; }
+};
 
-// Order-preserving integer keys, all > 0 (0 is free for "no expert"); NaN
-// counts as -inf, -0 as +0.
+// A choice value as it is compared: NaN counts as -inf, -0 as +0.
+__device__ __forceinline__ float route_clean(float v) { return isnan(v) ? -INFINITY : v + 0.0f; }
+__device__ __forceinline__ double route_clean(double v) { return isnan(v) ? -(double)INFINITY : v + 0.0; }
+
+// Order-preserving integer keys of clean values, all > 0 (0 is free for "none").
 __device__ __forceinline__ uint32_t route_key(float v) {
-    v = isnan(v) ? -INFINITY : v + 0.0f;
     const uint32_t b = __float_as_uint(v);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t route_key(double v) {
-    v = isnan(v) ? -(double)INFINITY : v + 0.0;
     const uint64_t b = (uint64_t)__double_as_longlong(v);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
+__device__ __forceinline__ float route_val(uint32_t k) {   // the value of a 32-bit key
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ float route_val(uint64_t) { return 0.0f; }   // (never asked)
 
 __device__ __forceinline__ uint32_t route_max(uint32_t v) { return __reduce_max_sync(MOE_FULL, v); }
 __device__ __forceinline__ uint64_t route_max(uint64_t v) {
@@ -72,174 +83,301 @@ __device__ __forceinline__ uint64_t route_max(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
+// The score of this lane's group: the largest clean value, or with group_top 2
+// the sum of the two largest.
+template <typename V, int J>
+__device__ __forceinline__ V route_group(const V (&c)[J], int count, const RouteSpec &s) {
+    V b1 = -(V)INFINITY, b2 = b1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const V v = j < count ? c[j] : -(V)INFINITY;
+        b2 = max(b2, min(b1, v));
+        b1 = max(b1, v);
+    }
+    for (int off = 1; off < 1 << s.log_lanes; off <<= 1) {
+        const V o1 = __shfl_xor_sync(MOE_FULL, b1, off), o2 = __shfl_xor_sync(MOE_FULL, b2, off);
+        b2 = max(min(b1, o1), max(b2, o2));
+        b1 = max(b1, o1);
+    }
+    return route_clean(s.group_top == 2 && s.per > 1 ? b1 + b2 : b1);
+}
+
 // True when this lane's group (its key gk, the same in all its lanes) is among
 // the topk_group largest.
 template <typename K>
-__device__ __forceinline__ bool route_group_kept(const RouteSpec &s, K gk, int lane) {
-    const int g = lane / s.lanes;
+__device__ __forceinline__ bool route_group_kept(const RouteSpec &s, K gk, int group) {
     int before = 0;
     for (int o = 0; o < s.n_group; ++o) {
-        const K ok = __shfl_sync(MOE_FULL, gk, o * s.lanes);
-        before += ok > gk || (ok == gk && o < g) ? 1 : 0;
+        const K ok = __shfl_sync(MOE_FULL, gk, o << s.log_lanes);
+        before += ok > gk || (ok == gk && o < group) ? 1 : 0;
     }
     return before < s.topk_group;
 }
 
-// The k largest keys (0: not to be chosen) of the warp in order: lane r < k
-// gets the id of rank r and that expert's logit.
-template <typename K, int J>
-__device__ __forceinline__ void route_topk(const K (&key)[J], const float (&l)[J], const RouteSpec &s, int lane,
-                                           int &id_r, float &l_r) {
-    uint32_t taken = 0;
+// (key, j) before (okey, oj): the larger key, then the lower j
+__device__ __forceinline__ void route_cx(uint32_t &ka, int &ja, uint32_t &kb, int &jb) {
+    const bool swap = kb > ka || (kb == ka && jb < ja);
+    const uint32_t k = swap ? kb : ka;
+    const int j = swap ? jb : ja;
+    kb = swap ? ka : kb;
+    jb = swap ? ja : jb;
+    ka = k;
+    ja = j;
+}
+
+// The k largest keys (0: none) of the warp in order: returns rank r's expert in
+// lane r < k.  Up to eight keys per lane are sorted first (Batcher's odd-even
+// merge), so that a round looks at one key per lane; more are searched every
+// round.  With tol >= 0 the first k + 1 are compared, and -1 is returned when
+// two neighbours are within tol of each other: errors of tol / 2 could then
+// change the order.
+template <int J>
+__device__ __forceinline__ int route_topk(uint32_t (&key)[J], const RouteSpec &s, const RouteLane &me, int lane,
+                                          float tol = -1.0f) {
+    constexpr bool SORT = J <= 8;
+    int at[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) at[j] = j;
+    if constexpr (SORT) {
+#pragma unroll
+        for (int p = 1; p < J; p *= 2)
+#pragma unroll
+            for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+                for (int j = q % p; j <= J - 1 - q; j += 2 * q)
+#pragma unroll
+                    for (int i = 0; i < q; ++i)
+                        if (i + j + q < J && (i + j) / (2 * p) == (i + j + q) / (2 * p))
+                            route_cx(key[i + j], at[i + j], key[i + j + q], at[i + j + q]);
+    }
+    float last = INFINITY;
+    int id_r = 0;
     for (int r = 0; r < s.k; ++r) {
-        K best = 0;
-        float bl = 0.0f;
-        int bj = 0;
+        uint32_t best = key[0];
+        int bj = at[0];
+        if constexpr (!SORT) {
+#pragma unroll
+            for (int j = 1; j < J; ++j)
+                if (key[j] > best) { best = key[j]; bj = j; }
+        }
+        const uint32_t m = __reduce_max_sync(MOE_FULL, best);
+        const int id = (int)__reduce_min_sync(MOE_FULL, best == m ? (unsigned)me.expert(bj) : (unsigned)ROUTE_MAX_EXPERT);
+        if (tol >= 0.0f) {
+            const float v = route_val(m);
+            if (last - v <= tol) return -1;
+            last = v;
+        }
+        const bool mine = best == m && me.expert(bj) == id;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if constexpr (SORT) {   // the list moves up
+                key[j] = mine ? j + 1 < J ? key[j + 1 < J ? j + 1 : j] : 0u : key[j];
+                at[j] = mine && j + 1 < J ? at[j + 1 < J ? j + 1 : j] : at[j];
+            } else {
+                key[j] = mine && j == bj ? 0u : key[j];
+            }
+        }
+        if (lane == r) id_r = id;
+    }
+    if (tol >= 0.0f) {   // and the best of those left out
+        uint32_t best = key[0];
+        if constexpr (!SORT) {
+#pragma unroll
+            for (int j = 1; j < J; ++j) best = max(best, key[j]);
+        }
+        best = __reduce_max_sync(MOE_FULL, best);
+        if (best && last - route_val(best) <= tol) return -1;
+    }
+    return id_r;
+}
+
+// The same for 64-bit values of the lanes' `alive` experts.
+template <int J>
+__device__ __forceinline__ int route_topk(const double (&c)[J], uint32_t alive, const RouteSpec &s, const RouteLane &me,
+                                          int lane) {
+    int id_r = 0;
+    for (int r = 0; r < s.k; ++r) {
+        double best = 0.0;
+        int bj = -1;
 #pragma unroll
         for (int j = 0; j < J; ++j)
-            if (!(taken >> j & 1) && key[j] > best) { best = key[j]; bl = l[j]; bj = j; }
-        const K m = route_max(best);
-        const int e = best == m && m ? route_expert(s, lane, bj) : ROUTE_MAX_EXPERT;
-        const int id = (int)__reduce_min_sync(MOE_FULL, (unsigned)e);
-        const int owner = __ffs(__ballot_sync(MOE_FULL, e == id)) - 1;
-        if (lane == owner) taken |= 1u << bj;
-        bl = __shfl_sync(MOE_FULL, bl, owner);
-        if (lane == r) { id_r = id; l_r = bl; }
+            if ((alive >> j & 1) && (bj < 0 || c[j] > best)) { best = c[j]; bj = j; }
+        const uint64_t k = bj < 0 ? 0ull : route_key(best);
+        const uint32_t hi = __reduce_max_sync(MOE_FULL, (uint32_t)(k >> 32));
+        const uint32_t lo = __reduce_max_sync(MOE_FULL, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+        const bool top = k && k == ((uint64_t)hi << 32 | lo);
+        const int id = (int)__reduce_min_sync(MOE_FULL, top ? (unsigned)me.expert(bj) : (unsigned)ROUTE_MAX_EXPERT);
+        if (top && me.expert(bj) == id) alive &= ~(1u << bj);
+        if (lane == r) id_r = id;
     }
+    return id_r;
 }
 
-__device__ __forceinline__ double warp_sum_f64(double v) {
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(MOE_FULL, v, off);
-    return v;
-}
-
-// One token: l[j] the logit of expert route_expert(s, lane, j).  Lane r < k
-// gets rank r's id and weight.  With `prior`, delta is added to the choice
-// value of the experts that are resident (prior_resident), after the groups.
-//
-// Without bias and prior the choice values fall with the logits, which are
-// compared as they are.  Otherwise the scores are computed and compared in 64
-// bits: in 32 bits the rounding of 1 / (1 + e^-l) would decide between close
-// experts.  The weights are formed in 64 bits, once per chosen expert.
+// Selection by 32-bit choice values where their rounding cannot matter: -1 when
+// some value is not finite, or two neighbours among the first k + 1, or the last
+// kept and first dropped group, are closer than twice their error.  With u =
+// 2^-24, the error of a value c is at most 10 u max(1, |c|) for sigmoid (expf 4 u
+// of a value below 1, a division of 4 u, two additions) and 30 u max(1, |c|) for
+// softmax (the sum's up to 15 additions, too): 2^-20 and 2^-18 are taken.  A
+// sum of two has twice that and its own rounding.
 template <int J>
-__device__ __forceinline__ void route_warp(const float (&l)[J], const RouteSpec &s, const int32_t *table, int ns,
-                                           float delta, bool prior, const int32_t *pub, int lane, int &id_r,
-                                           float &w_r) {
-    static_assert(J <= 32, "one bit of a mask per expert of a lane");
-    float mx = -INFINITY;
-    bool nan = false;
+__device__ __forceinline__ int route_fast(const float (&l)[J], const RouteSpec &s, const RouteLane &me, float mx, int lane,
+                                          float &total) {
+    float c[J], b[J], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, big = 1.0f;
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < J; ++j) b[j] = s.bias && j < me.count ? s.bias[me.expert(j)] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) c[j] = expf(s.sigmoid ? -l[j] : l[j] - mx);
+    if (s.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) c[j] = __fdividef(1.0f, 1.0f + c[j]) + b[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < J; ++j) sum[j & 3] += j < me.count ? c[j] : 0.0f;
+        total = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        const float inv = 1.0f / total;
+#pragma unroll
+        for (int j = 0; j < J; ++j) c[j] = fmaf(c[j], inv, b[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const float v = j < me.count ? fabsf(c[j]) : 0.0f;
+        big = fmaxf(big, v);
+        ok = ok && v < INFINITY;
+    }
+    if (!__all_sync(MOE_FULL, ok)) return -1;
+    big = __uint_as_float(__reduce_max_sync(MOE_FULL, __float_as_uint(big)));   // (positive: ordered as integers)
+    const float err = big * (s.sigmoid ? 0x1p-20f : 0x1p-18f);
+    bool kept = true;
+    if (s.n_group > 1) {
+        const bool mine = me.group < s.n_group;
+        const uint32_t gk = route_key(route_group(c, me.count, s));
+        kept = route_group_kept(s, gk, me.group);
+        const uint32_t lo = __reduce_min_sync(MOE_FULL, mine && kept ? gk : 0xffffffffu);
+        const uint32_t hi = __reduce_max_sync(MOE_FULL, mine && !kept ? gk : 0u);
+        if (hi && route_val(lo) - route_val(hi) <= 6.0f * err) return -1;
+    }
+    uint32_t key[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) key[j] = kept && j < me.count ? route_key(c[j]) : 0u;
+    return route_topk(key, s, me, lane, 2.0f * err);
+}
+
+// Selection by 64-bit values, which a softmax with a NaN or +inf logit (bad)
+// makes NaN; with `prior`, delta is added to the experts that are resident
+// (prior_resident), after the groups.
+template <int J>
+__device__ __forceinline__ int route_exact(const float (&l)[J], const RouteSpec &s, const RouteLane &me, float mx, bool bad,
+                                           const int32_t *table, int ns, float delta, bool prior, const int32_t *pub,
+                                           int lane) {
+    double c[J], total = 0.0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        c[j] = 0.0;
+        if (j >= me.count) continue;
+        c[j] = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l[j])) : mx > -INFINITY ? exp((double)l[j] - (double)mx) : 0.0;
+        total += c[j];
+    }
+    double inv = 1.0;
+    if (!s.sigmoid) {
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(MOE_FULL, total, off);
+        inv = bad ? NAN : total == 0.0 ? 0.0 : 1.0 / total;
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j)
-        if (route_expert(s, lane, j) >= 0) {
-            nan |= isnan(l[j]);
-            mx = fmaxf(mx, l[j]);
-        }
+        if (j < me.count) c[j] = route_clean(c[j] * inv + (s.bias ? (double)s.bias[me.expert(j)] : 0.0));
+    const bool kept = s.n_group == 1 || route_group_kept(s, route_key(route_group(c, me.count, s)), me.group);
+    uint32_t alive = 0;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(MOE_FULL, mx, off));
-    nan = __any_sync(MOE_FULL, nan) || mx == INFINITY;   // then every softmax score is NaN
-    double total = 0.0;   // of e^(l - mx) over all experts, where it is needed
-    float l_r = 0.0f;
-    id_r = 0;
-    if (!s.bias && !prior && (s.n_group == 1 || s.group_top == 1)) {
-        uint32_t key[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) key[j] = route_expert(s, lane, j) >= 0 ? route_key(l[j]) : 0u;
-        if (s.n_group > 1) {
-            uint32_t gk = 0;
-#pragma unroll
-            for (int j = 0; j < J; ++j) gk = max(gk, key[j]);
-            for (int off = 1; off < s.lanes; off <<= 1) gk = max(gk, __shfl_xor_sync(MOE_FULL, gk, off));
-            if (!route_group_kept(s, gk, lane)) {
-#pragma unroll
-                for (int j = 0; j < J; ++j) key[j] = 0u;
-            }
-        }
-        route_topk(key, l, s, lane, id_r, l_r);
-        if (!s.sigmoid && !s.renorm) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-                if (route_expert(s, lane, j) >= 0 && mx > -INFINITY) sum += expf(l[j] - mx);
-            total = warp_sum_f64((double)sum);
-        }
-    } else {
-        double c[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            c[j] = 0.0;
-            if (route_expert(s, lane, j) < 0) continue;
-            c[j] = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l[j])) : mx > -INFINITY ? exp((double)l[j] - (double)mx) : 0.0;
-            total += c[j];
-        }
-        if (!s.sigmoid) {
-            total = warp_sum_f64(total);
-            const double inv = total == 0.0 ? 0.0 : 1.0 / total;
-#pragma unroll
-            for (int j = 0; j < J; ++j) c[j] = nan ? NAN : c[j] * inv;
-        }
-        uint64_t key[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = route_expert(s, lane, j);
-            if (s.bias && e >= 0) c[j] += (double)s.bias[e];
-            key[j] = e >= 0 ? route_key(c[j]) : 0ull;
-        }
-        if (s.n_group > 1) {
-            double b1 = -(double)INFINITY, b2 = b1;   // the two largest of the group
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                if (route_expert(s, lane, j) < 0) continue;
-                const double v = isnan(c[j]) ? -(double)INFINITY : c[j];
-                b2 = fmax(b2, fmin(b1, v));
-                b1 = fmax(b1, v);
-            }
-            for (int off = 1; off < s.lanes; off <<= 1) {
-                const double o1 = __shfl_xor_sync(MOE_FULL, b1, off), o2 = __shfl_xor_sync(MOE_FULL, b2, off);
-                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
-                b1 = fmax(b1, o1);
-            }
-            if (!route_group_kept(s, route_key(s.group_top == 2 && s.per > 1 ? b1 + b2 : b1), lane)) {
-#pragma unroll
-                for (int j = 0; j < J; ++j) key[j] = 0ull;
-            }
-        }
-        if (prior) {
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int e = route_expert(s, lane, j);
-                if (key[j] && prior_resident(table, ns, pub, e)) key[j] = route_key(c[j] + (double)delta);
-            }
-        }
-        route_topk(key, l, s, lane, id_r, l_r);
+    for (int j = 0; j < J; ++j) {
+        if (!kept || j >= me.count) continue;
+        alive |= 1u << j;
+        if (prior && prior_resident(table, ns, pub, me.expert(j))) c[j] += (double)delta;
     }
-    double v = 0.0;
-    if (lane < s.k) {
-        if (s.sigmoid) v = 1.0 / (1.0 + exp(-(double)l_r));
-        else if (nan) v = NAN;
-        else if (mx > -INFINITY) v = exp((double)l_r - (double)mx);
-    }
-    if (s.renorm) total = warp_sum_f64(v);
-    if (s.renorm || !s.sigmoid) v = total == 0.0 ? 0.0 : v / total;
-    w_r = (float)(v * (double)s.scale);
+    return route_topk(c, alive, s, me, lane);
 }
 
 __device__ __forceinline__ float route_load(const float *p) { return *p; }
 __device__ __forceinline__ float route_load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float route_load(const __half *p) { return __half2float(*p); }
 
-// route_warp over a token's logits in memory (shared or global).
+// One token's ids and weights (lane r < k gets rank r's) from its logits in
+// shared or global memory, at most J per lane.
+//
+// Without bias and prior the choice values fall with the logits, which are
+// compared as they are.  Otherwise 32-bit scores decide where they are far
+// enough apart (route_fast: about 998 tokens in 1000), and 64-bit scores where
+// their rounding could decide between two experts.
+//
+// The weights are formed in 32 bits (expf 4 u with the rounding of l - mx taken
+// back, k - 1 additions in five levels, two divisions, scale: below 20 u); where
+// their sum is so small that scores may have underflowed, in 64 bits.
 template <int J, typename T>
 __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s, const int32_t *table, int ns,
                                                float delta, bool prior, const int32_t *pub, int lane, int &id_r,
                                                float &w_r) {
-    float l[J];
+    static_assert(J <= 32, "one bit of a mask per expert of a lane");
+    const RouteLane me(s, lane);
+    float l[J], mx = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < J; ++j) l[j] = j < me.count ? route_load(row + me.expert(j)) : -INFINITY;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const int e = route_expert(s, lane, j);
-        l[j] = e >= 0 ? route_load(row + e) : 0.0f;
+        bad = bad || isnan(l[j]);
+        mx = fmaxf(mx, l[j]);
     }
-    route_warp<J>(l, s, table, ns, delta, prior, pub, lane, id_r, w_r);
+    mx = route_val(__reduce_max_sync(MOE_FULL, route_key(mx)));
+    bad = __any_sync(MOE_FULL, bad) || mx == INFINITY;   // then every softmax score is NaN
+    float total = 0.0f;   // of e^(l - mx) over all experts
+    if (!s.bias && !prior && (s.n_group == 1 || s.group_top == 1)) {
+        uint32_t key[J];
+        bool kept = true;
+        if (s.n_group > 1) {
+            float c[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) c[j] = route_clean(l[j]);
+            kept = route_group_kept(s, route_key(route_group(c, me.count, s)), me.group);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) key[j] = kept && j < me.count ? route_key(route_clean(l[j])) : 0u;
+        id_r = route_topk(key, s, me, lane);
+    } else {
+        id_r = prior || bad ? -1 : route_fast<J>(l, s, me, mx, lane, total);
+        if (__any_sync(MOE_FULL, id_r < 0))
+            id_r = route_exact<J>(l, s, me, mx, bad, table, ns, delta, prior, pub, lane);
+    }
+    if (!s.sigmoid && !s.renorm) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) sum[j & 3] += j < me.count && mx > -INFINITY ? expf(l[j] - mx) : 0.0f;
+        total = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+    const float l_r = lane < s.k ? route_load(row + id_r) : -INFINITY;
+    float v = 0.0f;
+    if (s.sigmoid) v = lane < s.k ? 1.0f / (1.0f + expf(-l_r)) : 0.0f;
+    else if (bad) v = NAN;
+    else if (mx > -INFINITY && l_r > -INFINITY) {
+        const float d = l_r - mx, t = d - l_r;              // l_r - mx = d + rest exactly
+        const float rest = (l_r - (d - t)) - (mx + t);
+        v = expf(d);
+        if (v > 0.0f) v = fmaf(v, rest, v);                 // (d may be -inf)
+    }
+    if (s.renorm) total = warp_sum(lane < s.k ? v : 0.0f);
+    if (s.renorm && total < 1e-20f) {
+        double x = 0.0, sum;
+        if (lane < s.k)
+            x = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l_r)) : mx > -INFINITY ? exp((double)l_r - (double)mx) : 0.0;
+        sum = x;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(MOE_FULL, sum, off);
+        v = sum == 0.0 ? 0.0f : (float)(x / sum);
+    } else if (s.renorm || !s.sigmoid) {
+        v = total == 0.0f ? 0.0f : v / total;
+    }
+    w_r = v * s.scale;
 }
 
 }  // namespace moe

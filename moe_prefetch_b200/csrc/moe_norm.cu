@@ -14,195 +14,371 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace moe {
 
-// VEC values of one type, loaded and stored with 16-byte accesses (VEC 8) or
-// one by one (VEC 1).
-__device__ __forceinline__ void norm_load(const float *p, float (&v)[1]) { v[0] = *p; }
-__device__ __forceinline__ void norm_load(const __nv_bfloat16 *p, float (&v)[1]) { v[0] = __bfloat162float(*p); }
-__device__ __forceinline__ void norm_load(const __half *p, float (&v)[1]) { v[0] = __half2float(*p); }
-__device__ __forceinline__ void norm_load(const float *p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void norm_load(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+// VEC values of one type as they are in memory: one by one (VEC 1), four (16
+// bytes of fp32, 8 of a 16-bit type) or eight of a 16-bit type.  A warp's
+// access then covers neighbouring whole sectors.
+template <typename T, int VEC> struct NormRaw;
+template <typename T> struct NormRaw<T, 1> {
+    T u;
+    __device__ __forceinline__ void load(const T *p) { u = *p; }
+    __device__ __forceinline__ void zero() { u = T(0.0f); }
+    __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = (float)u; }
+};
+template <> struct NormRaw<float, 4> {
+    float4 a;
+    __device__ __forceinline__ void load(const float *p) { a = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void zero() { a = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
+};
+template <> struct NormRaw<float, 8> {   // the norm weights beside 16-bit rows
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = reinterpret_cast<const float4 *>(p)[0];
+        b = reinterpret_cast<const float4 *>(p)[1];
     }
-}
-__device__ __forceinline__ void norm_load(const __half *p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
-}
-__device__ __forceinline__ void norm_store(float *p, const float (&v)[1]) { *p = v[0]; }
-__device__ __forceinline__ void norm_store(__nv_bfloat16 *p, const float (&v)[1]) { *p = __float2bfloat16(v[0]); }
-__device__ __forceinline__ void norm_store(__half *p, const float (&v)[1]) { *p = __float2half(v[0]); }
-__device__ __forceinline__ void norm_store(float *p, const float (&v)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void norm_store(__nv_bfloat16 *p, const float (&v)[8]) {
-    uint4 a;
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t *>(&b);
+};
+template <typename T, int VEC> struct NormRaw {   // 16 bits, VEC 4 or 8
+    uint32_t u[VEC / 2];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC == 8) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(p);
+            u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2 *>(p);
+            u[0] = a.x; u[1] = a.y;
+        }
     }
-    a.x = u[0]; a.y = u[1]; a.z = u[2]; a.w = u[3];
-    *reinterpret_cast<uint4 *>(p) = a;
-}
-__device__ __forceinline__ void norm_store(__half *p, const float (&v)[8]) {
-    uint4 a;
-    uint32_t u[4];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t *>(&b);
+        for (int i = 0; i < VEC / 2; ++i) u[i] = 0;
     }
-    a.x = u[0]; a.y = u[1]; a.z = u[2]; a.w = u[3];
-    *reinterpret_cast<uint4 *>(p) = a;
+    __device__ __forceinline__ void get(float (&v)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void norm_load(const T *p, float (&v)[VEC]) {
+    NormRaw<T, VEC> u;
+    u.load(p);
+    u.get(v);
+}
+__device__ __forceinline__ uint32_t norm_pack(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t norm_pack(float a, float b, __half) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void norm_store(T *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = T(v[0]);
+    else if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (VEC == 4)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(norm_pack(v[0], v[1], T()), norm_pack(v[2], v[3], T()));
+    else
+        *reinterpret_cast<uint4 *>(p) = make_uint4(norm_pack(v[0], v[1], T()), norm_pack(v[2], v[3], T()),
+                                                   norm_pack(v[4], v[5], T()), norm_pack(v[6], v[7], T()));
 }
 
-// The CTA's sum of v; `part` [33] is used by this call alone.  Warp totals are
-// added in warp order by every thread, so the result does not depend on timing.
+// The CTA's sum of v; `part` [32] is this sum's alone until the CTA's next
+// barrier.  Every thread adds the warps' totals in the same order, so the
+// result does not depend on timing.
 __device__ __forceinline__ float norm_cta_sum(float v, float *part) {
     v = warp_sum(v);
     const int nw = blockDim.x >> 5;
     if (nw == 1) return v;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
+    if (nw <= 8) {   // (part past nw is zero: k_block_norm clears it)
+        const float4 a = reinterpret_cast<const float4 *>(part)[0], b = reinterpret_cast<const float4 *>(part)[1];
+        return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    }
     v = (int)(threadIdx.x & 31) < nw ? part[threadIdx.x & 31] : 0.0f;
     return warp_sum(v);
 }
 
-// One CTA per row; thread i holds the chunks of VEC values at VEC * (i + c *
-// blockDim.x), c < V.  SRC 0: y rows of type TY; 1: the combine of fp32 rows.
-// Everything the row needs is loaded before the first sum, so that one memory
-// latency covers it.
-template <typename TR, typename TY, int VEC, int V, int SRC>
-__global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
-    __shared__ float part[2][32];
-    const int t = blockIdx.x;
+// 1 / (1 + e^-v): expf and a reciprocal of one ulp (the argument is at least 1)
+__device__ __forceinline__ float norm_sigmoid(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-v)));
+    return r;
+}
+
+// B bytes (8 or 16) into shared memory without a register.
+template <int B>
+__device__ __forceinline__ void norm_copy(void *dst, const void *src) {
+    if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// A CTA takes rows blockIdx.x, + gridDim.x, ...; thread i holds the chunks of VEC
+// values at VEC * (i + c * blockDim.x), c < V.  SRC 0: y rows of type TY; 1: the
+// combine of fp32 rows.  The norm weights stay in registers over the rows.  With
+// S > 0, r, y and a full gate come through a ring of S rows in dynamic shared
+// memory, each thread copying and reading its own chunks (so the ring needs no
+// barrier): the kernel is bound by memory, and S - 1 rows are on their way while
+// one is in its two sums.
+template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(NormArgs a) {
+    static_assert(S == 0 || (SRC == 0 && VEC > 1), "the ring holds aligned rows");
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ __align__(16) float part[2][32];
     const int H = a.n_embd;
     const float inv_h = 1.0f / (float)H;   // each square is scaled first: the sum overflows only where the mean does
-    float y[V][VEC], r[V][VEC], g[V][VEC], po[V][VEC];
-    const TR *rr = (const TR *)a.r + (int64_t)t * a.ld_r;
-    float gt[1] = {0.0f};
-    if (a.gate_kind == NORM_GATE_TOKEN) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate, gt);
+    auto at = [&](int c) { return VEC * ((int)threadIdx.x + c * (int)blockDim.x); };
+    if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
+    if (threadIdx.x + 32 < 64 && blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
+    __syncthreads();
+    float post[V][VEC], pre[V][VEC];        // weight + offset
+    auto load_weights = [&]() {
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-        const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
+        for (int c = 0; c < V; ++c) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) y[c][i] = r[c][i] = po[c][i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) g[c][i] = 0.0f;
-        if (h >= H) continue;
-        norm_load(rr + h, r[c]);
-        if (SRC == 0 && a.y) norm_load((const TY *)a.y + (int64_t)t * a.ld_y + h, y[c]);
-        if (a.gate_kind == NORM_GATE_FULL) norm_load((const TY *)a.gate + (int64_t)t * a.ld_gate + h, g[c]);
-        else if (a.gate_kind == NORM_GATE_CHANNEL) norm_load((const float *)a.gate + h, g[c]);
-        if (a.post) norm_load(a.post + h, po[c]);
-    }
-    if (SRC == 1) {
-        // the chain of k_combine: fma from 0 in rank order, then + add.  Four
-        // rows are in flight at a time.
-        const float *rows = (const float *)a.y;
-        const int32_t *pos = a.pos + (int64_t)t * a.k;
-        const float *w = a.w + (int64_t)t * a.k;
-        constexpr int U = VEC * V <= 8 ? 4 : 2;
-        for (int j0 = 0; j0 < a.k; j0 += U) {
-            float v[U][V][VEC], wj[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int at = j0 + u < a.k ? pos[j0 + u] : -1;
-                wj[u] = j0 + u < a.k ? w[j0 + u] : 0.0f;
-#pragma unroll
-                for (int c = 0; c < V; ++c) {
-                    const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[u][c][i] = 0.0f;
-                    if (h < H && at >= 0 && at < a.n_rows) norm_load(rows + (int64_t)at * a.ld_y + h, v[u][c]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j0 + u < a.k) {
-#pragma unroll
-                    for (int c = 0; c < V; ++c)
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) y[c][i] = __fmaf_rn(wj[u], v[u][c][i], y[c][i]);
-                }
-        }
-        if (a.add) {
-#pragma unroll
-            for (int c = 0; c < V; ++c) {
-                const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
-                if (h < H) {
-                    float v[VEC];
-                    norm_load(a.add + (int64_t)t * H + h, v);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) y[c][i] = __fadd_rn(y[c][i], v[i]);
-                }
-            }
-        }
-    }
-    if (a.post) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) ss = fmaf(y[c][i] * inv_h, y[c][i], ss);
-        const float inv = 1.0f / sqrtf(norm_cta_sum(ss, part[0]) + a.eps);
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) y[c][i] *= inv * (po[c][i] + a.offset);
-    }
-    if (a.gate_kind != NORM_GATE_NONE) {
-#pragma unroll
-        for (int c = 0; c < V; ++c)
+            for (int i = 0; i < VEC; ++i) post[c][i] = pre[c][i] = 0.0f;
+            if (at(c) < H && a.post) norm_load(a.post + at(c), post[c]);
+            if (at(c) < H && a.pre) norm_load(a.pre + at(c), pre[c]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float v = a.gate_kind == NORM_GATE_TOKEN ? gt[0] : g[c][i];
-                y[c][i] *= a.sigmoid ? 1.0f / (1.0f + expf(-v)) : v;
+                post[c][i] += a.offset;
+                pre[c][i] = a.pre ? pre[c][i] + a.offset : 1.0f;
             }
+        }
+    };
+    if (SRC == 0) load_weights();
+    NormRaw<TR, VEC> r_raw[V];
+    NormRaw<TY, VEC> y_raw[V], g_raw[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {   // what is not loaded below stays zero
+        r_raw[c].zero();
+        y_raw[c].zero();
+        g_raw[c].zero();
     }
-    float ss = 0.0f;
-    TR *ro = (TR *)a.r_out + (int64_t)t * a.ld_ro;
+    float g_tok = 1.0f;
+    auto load_row = [&](int64_t t) {
+        const TY *gr = (const TY *)a.gate + t * a.ld_gate;   // (read where the gate is per token or full)
+        if (a.gate_kind == NORM_GATE_TOKEN) {
+            NormRaw<TY, 1> u;
+            float v[1];
+            u.load(gr);
+            u.get(v);
+            g_tok = v[0];
+        }
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-        const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
+        for (int c = 0; c < V; ++c) {
+            if (at(c) >= H) continue;
+            r_raw[c].load((const TR *)a.r + t * a.ld_r + at(c));
+            if (SRC == 0 && a.y) y_raw[c].load((const TY *)a.y + t * a.ld_y + at(c));
+            if (a.gate_kind == NORM_GATE_FULL) g_raw[c].load(gr + at(c));
+        }
+    };
+    // the ring: per row r, y, and the gate where it is full
+    const int row_bytes = H * (int)(sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1));
+    auto copy_row = [&](int64_t t, int stage) {
+        uint8_t *dst = ring + stage * row_bytes;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r[c][i] = h < H ? fmaf(a.scale, y[c][i], r[c][i]) : 0.0f;
+        for (int c = 0; c < V; ++c) {
+            const int h = at(c);
+            if (h >= H) continue;
+            norm_copy<VEC * (int)sizeof(TR)>(dst + h * (int)sizeof(TR), (const TR *)a.r + t * a.ld_r + h);
+            uint8_t *dy = dst + H * (int)sizeof(TR) + h * (int)sizeof(TY);
+            if (a.y) norm_copy<VEC * (int)sizeof(TY)>(dy, (const TY *)a.y + t * a.ld_y + h);
+            if (a.gate_kind == NORM_GATE_FULL)
+                norm_copy<VEC * (int)sizeof(TY)>(dy + H * (int)sizeof(TY), (const TY *)a.gate + t * a.ld_gate + h);
+        }
+    };
+    auto read_row = [&](int64_t t, int stage) {
+        const uint8_t *src = ring + stage * row_bytes;
+        if (a.gate_kind == NORM_GATE_TOKEN) {
+            float v[1];
+            norm_load((const TY *)a.gate + t * a.ld_gate, v);
+            g_tok = v[0];
+        }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
-        if (h < H && a.r_out) norm_store(ro + h, r[c]);
-        if (h < H && a.x && a.pre) norm_load(a.pre + h, po[c]);
+        for (int c = 0; c < V; ++c) {
+            const int h = at(c);
+            if (h >= H) continue;
+            r_raw[c].load((const TR *)src + h);
+            const TY *sy = (const TY *)(src + H * (int)sizeof(TR)) + h;
+            if (a.y) y_raw[c].load(sy);
+            if (a.gate_kind == NORM_GATE_FULL) g_raw[c].load(sy + H);
+        }
+    };
+    if (S) {
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) {
+            if (blockIdx.x + (int64_t)i * gridDim.x < a.n_tok) copy_row(blockIdx.x + (int64_t)i * gridDim.x, i);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
     }
-    if (!a.x) return;
-    const float inv = 1.0f / sqrtf(norm_cta_sum(ss, part[1]) + a.eps);
-    TY *xo = (TY *)a.x + (int64_t)t * a.ld_x;
+    int stage = 0;
+    for (int64_t t = blockIdx.x; t < a.n_tok; t += gridDim.x) {
+        if (S) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S > 1 ? S - 2 : 0) : "memory");
+            read_row(t, stage);
+            const int64_t next = t + (int64_t)(S - 1) * gridDim.x;
+            if (next < a.n_tok) copy_row(next, stage == 0 ? S - 1 : stage - 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            stage = stage + 1 == S ? 0 : stage + 1;
+        } else {
+            load_row(t);
+        }
+        float y[V][VEC], r[V][VEC], f[V][VEC];
+        const float g_now = g_tok;
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-        const int h = VEC * ((int)threadIdx.x + c * (int)blockDim.x);
+        for (int c = 0; c < V; ++c) {
+            r_raw[c].get(r[c]);
+            y_raw[c].get(y[c]);
+            g_raw[c].get(f[c]);
+        }
+        if (SRC == 1) {
+            // the chain of k_combine: fma from 0 in rank order, then + add; U rows
+            // are in flight at a time
+            const float *rows = (const float *)a.y;
+            const int32_t *pos = a.pos + t * a.k;
+            const float *w = a.w + t * a.k;
+            constexpr int U = THREADS == 256 && VEC > 1 ? 4 : 2;
+            for (int j0 = 0; j0 < a.k; j0 += U) {
+                float v[U][V][VEC], wj[U];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r[c][i] *= inv * (a.pre ? po[c][i] + a.offset : 1.0f);
-        if (h < H) norm_store(xo + h, r[c]);
+                for (int u = 0; u < U; ++u) {
+                    const int q = j0 + u < a.k ? pos[j0 + u] : -1;
+                    wj[u] = j0 + u < a.k ? w[j0 + u] : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < V; ++c) {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) v[u][c][i] = 0.0f;
+                        if (at(c) < H && q >= 0 && q < a.n_rows) norm_load(rows + (int64_t)q * a.ld_y + at(c), v[u][c]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (j0 + u < a.k) {
+#pragma unroll
+                        for (int c = 0; c < V; ++c)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) y[c][i] = __fmaf_rn(wj[u], v[u][c][i], y[c][i]);
+                    }
+            }
+            load_weights();   // (one row per CTA: no earlier than they are needed)
+            if (a.add) {
+#pragma unroll
+                for (int c = 0; c < V; ++c)
+                    if (at(c) < H) {
+                        float v[VEC];
+                        norm_load(a.add + t * H + at(c), v);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) y[c][i] = __fadd_rn(y[c][i], v[i]);
+                    }
+            }
+        }
+        // the gate's factor
+        if (a.gate_kind == NORM_GATE_TOKEN) {
+            const float v = a.sigmoid ? norm_sigmoid(g_now) : g_now;
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] = v;
+        } else if (a.gate_kind != NORM_GATE_NONE) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                if (a.gate_kind == NORM_GATE_CHANNEL && at(c) < H) norm_load((const float *)a.gate + at(c), f[c]);
+                if (a.sigmoid) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
+                }
+            }
+        }
+        float by = a.scale;   // times scale, times post's 1 / sqrt
+        if (a.post) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) ss = fmaf(y[c][i] * inv_h, y[c][i], ss);
+            by = a.scale * rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
+            if (a.gate_kind == NORM_GATE_NONE) {
+#pragma unroll
+                for (int c = 0; c < V; ++c)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f[c][i] = post[c][i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < V; ++c)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f[c][i] *= post[c][i];
+            }
+        }
+        float ss = 0.0f;
+        TR *ro = (TR *)a.r_out + t * a.ld_ro;
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            if (at(c) >= H) continue;   // (r is 0 there and adds nothing)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                r[c][i] = a.post || a.gate_kind != NORM_GATE_NONE ? fmaf(y[c][i] * by, f[c][i], r[c][i])
+                                                                  : fmaf(by, y[c][i], r[c][i]);
+                ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
+            }
+            if (a.r_out) norm_store(ro + at(c), r[c]);
+        }
+        if (!a.x) {
+            __syncthreads();   // part[0] is read before the next row writes it
+            continue;
+        }
+        const float inv = rsqrtf(norm_cta_sum(ss, part[1]) + a.eps);
+        TY *xo = (TY *)a.x + t * a.ld_x;
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            if (at(c) >= H) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) r[c][i] *= inv * pre[c][i];
+            norm_store(xo + at(c), r[c]);
+        }
+        if (!a.post) __syncthreads();   // part[1] is read before the next row writes it
     }
+}
+
+template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
+static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
+    // as many CTAs as the GPU holds, at most one per row; the combine takes a CTA
+    // per row, since its own loads are many enough
+    int dev = 0, sms = 0;
+    cudaError_t e;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    int per_sm = 1024 / threads;
+    const size_t smem = (size_t)S * a.n_embd * (sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1));
+    if (S) {
+        per_sm = std::min(per_sm, (int)(220 * 1024 / (smem + 2048)));
+        if (smem > 40 * 1024 &&
+            (e = cudaFuncSetAttribute(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
+            return e;
+    }
+    per_sm = std::min(16, std::max(1, per_sm));
+    k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>
+        <<<SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads, smem, s>>>(a);
+    return cudaGetLastError();
 }
 
 template <typename TR, typename TY, int VEC, int SRC>
@@ -213,9 +389,10 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const bool wide = chunks > 1024 * V8;
     const int per = wide ? 2 * V8 : V8;
     const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;
-    if (wide) k_block_norm<TR, TY, VEC, 2 * V8, SRC><<<a.n_tok, threads, 0, s>>>(a);
-    else k_block_norm<TR, TY, VEC, V8, SRC><<<a.n_tok, threads, 0, s>>>(a);
-    return cudaGetLastError();
+    constexpr bool RING = VEC > 1 && SRC == 0;   // up to 12 bytes a value: 3 rows of 2048, 2 of 8192
+    if (wide) return norm_launch<TR, TY, VEC, 2 * V8, SRC, 1024, 0>(a, threads, s);
+    return threads > 256 ? norm_launch<TR, TY, VEC, V8, SRC, 1024, RING ? 2 : 0>(a, threads, s)
+                         : norm_launch<TR, TY, VEC, V8, SRC, 256, RING ? 3 : 0>(a, threads, s);
 }
 
 template <typename TR, typename TY>
@@ -224,6 +401,7 @@ static cudaError_t norm_types(const NormArgs &a, cudaStream_t s) {
     auto al = [](const void *p, int64_t ld, size_t size) {
         return !p || (((uintptr_t)p | (uintptr_t)(ld * (int64_t)size)) & 15) == 0;
     };
+    constexpr int VEC = std::is_same<TR, float>::value ? 4 : 8;
     const bool vec = a.n_embd % 8 == 0 && al(a.r, a.ld_r, sizeof(TR)) && al(a.r_out, a.ld_ro, sizeof(TR)) &&
                      al(a.y, a.ld_y, sizeof(TY)) && al(a.x, a.ld_x, sizeof(TY)) && al(a.add, a.n_embd, 4) &&
                      al(a.post, 0, 4) && al(a.pre, 0, 4) &&
@@ -231,11 +409,11 @@ static cudaError_t norm_types(const NormArgs &a, cudaStream_t s) {
                       al(a.gate, a.gate_kind == NORM_GATE_FULL ? a.ld_gate : 0, sizeof(TY)));
     if (a.pos) {   // the expert rows of a layer are fp32
         if constexpr (std::is_same<TR, float>::value && std::is_same<TY, float>::value)
-            return vec ? norm_go<TR, TY, 8, 1>(a, s) : norm_go<TR, TY, 1, 1>(a, s);
+            return vec ? norm_go<TR, TY, VEC, 1>(a, s) : norm_go<TR, TY, 1, 1>(a, s);
         else
             return cudaErrorInvalidValue;
     }
-    return vec ? norm_go<TR, TY, 8, 0>(a, s) : norm_go<TR, TY, 1, 0>(a, s);
+    return vec ? norm_go<TR, TY, VEC, 0>(a, s) : norm_go<TR, TY, 1, 0>(a, s);
 }
 
 cudaError_t launch_block_norm(const NormArgs &a, int dt_r, int dt_y, cudaStream_t s) {

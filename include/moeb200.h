@@ -593,14 +593,15 @@ typedef struct moe_norm {
 /* r, r_out [n_tok][n_embd] of r_dtype; y, x and a token or full gate of dtype.
  * r_dtype is MOE_DTYPE_F32 or dtype.  y NULL: r' = r (then no post, no gate).
  * r_out NULL (r' not wanted) or x NULL (no second norm), not both.  r_out may be
- * r, and x may be y. */
+ * r, and x may be y or, without r_out, r; other overlaps are not allowed. */
 int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r, const void *y, int dtype,
                    int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok, void *stream);
 
 /* The same with y[t] = sum over j in order of w[t][j] * y_rows[pos[t][j]], then
  * + add[t] when given: moe_ep_combine's sum, bit for bit, never written to
  * memory.  All fp32; pos / w [n_tok][k], add [n_tok][n_embd].  A pos outside
- * [0, n_rows) adds nothing (-1: an empty pair). */
+ * [0, n_rows) adds nothing (-1: an empty pair).  r_out may be r; no output
+ * overlaps y_rows. */
 int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const float *y_rows, int64_t ld_rows,
                      int n_rows, const int32_t *pos, const float *w, int k, const float *add, float *r_out,
                      int64_t ld_ro, float *x, int64_t ld_x, int n_tok, void *stream);
@@ -623,7 +624,7 @@ typedef struct moe_adapters {
 } moe_adapters;
 
 /* out[t] = y[t] + scale[i] * B_i (A_i x[t]) with i = ids[t] (device); y NULL
- * counts as 0, out may be y.  A row whose id is outside [0, n_adapters) gets
+ * counts as 0; out may be y, never x.  A row whose id is outside [0, n_adapters) gets
  * y[t] (-1: a request without an adapter).  Types: x fp32, y and out fp32; or x
  * of the weights' type, y and out of that type or fp32.  A x stays in fp32. */
 int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *x, int x_dtype, int64_t ld_x,

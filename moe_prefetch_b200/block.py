@@ -6,7 +6,7 @@ calls (the rule, the norm weights, the adapters laid out for the kernels) and
 are called on device tensors.  ``MoeStack.set_routing`` gives a layer a routing
 rule, and ``MoeStack.block_forward`` runs a whole layer with all three.
 
-Every call takes its work to the tensors' device, on that device's current
+They are for inference: no call records a gradient.  Every call takes its work to the tensors' device, on that device's current
 stream or on ``stream``; nothing waits for the host, and the calls can be
 captured in a CUDA graph.  With ``stream`` the caller orders it after the
 producers of the inputs; the outputs are allocated for that stream.
@@ -73,9 +73,8 @@ def _on_stream(call, stream, tensors):
     return out
 
 
-def _elsewhere(index):
-    """True when the tensors' device is not the current one."""
-    return index != torch.cuda.current_device()
+# the current device's index (a call on tensors of another one enters it first)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class Routing:
@@ -109,7 +108,7 @@ class Routing:
         if stream is not None:
             return _on_stream(lambda: self(logits, out), stream, (logits, self.bias) + (out or ()))
         index = logits.get_device()
-        if index >= 0 and _elsewhere(index):
+        if index >= 0 and index != _current_device():
             with torch.cuda.device(index):
                 return self(logits, out)
         ld = _rows(logits, "logits", self.n_expert)
@@ -154,17 +153,15 @@ class BlockNorm:
         for name, t in (("post", self.post), ("pre", self.pre)):
             if t is not None and (t.shape != (n_embd,) or t.dtype != torch.float32 or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous fp32 [{n_embd}]")
+        self.device = next((t.device for t in (self.post, self.pre) if t is not None), None)
+        if None not in (self.post, self.pre) and self.post.device != self.pre.device:
+            raise ValueError(f"post is on {self.post.device}, pre on {self.pre.device}")
         self.nm = MoeNorm(n_embd, GATE_NONE, ACTS[gate_act], scale, eps, weight_offset,
                           None if self.post is None else self.post.data_ptr(),
                           None if self.pre is None else self.pre.data_ptr(), None, 0)
         self.nm_ref = C.byref(self.nm)
         check(self.lib.moe_block_norm(self.nm_ref, None, 0, n_embd, None, 0, n_embd, None, n_embd, None, n_embd,
                                       0, None), None, "moe_block_norm")
-
-    def _weights_on(self, device):
-        for t in (self.post, self.pre):
-            if t is not None and t.device != device:
-                raise ValueError(f"the norm's weights are on {t.device}, expected {device}")
 
     def with_gate(self, gate, n, dtype, device):
         """The moe_norm of one call; gate None, [n, 1] (per row), [n_embd] (per
@@ -190,12 +187,8 @@ class BlockNorm:
             nm.gate_kind = GATE_FULL
         return nm
 
-    def _outputs(self, r, dtype, out):
+    def _check_out(self, r, dtype, out):
         n, h = r.shape
-        if out is None:
-            device = r.device
-            ro = torch.empty(n, h, dtype=r.dtype, device=device)
-            return ro, torch.empty(n, h, dtype=dtype, device=device) if self.with_x else None, h, h
         ro, x = out
         if (x is not None) != self.with_x or ro is None and x is None:
             raise ValueError("out must be (r', x), with None for x without a second norm")
@@ -218,7 +211,7 @@ class BlockNorm:
             return _on_stream(lambda: self(r, y, gate, out), stream,
                               (r, y, gate, self.post, self.pre) + (out or ()))
         index = r.get_device()
-        if index >= 0 and _elsewhere(index):
+        if index >= 0 and index != _current_device():
             with torch.cuda.device(index):
                 return self(r, y, gate, out)
         ld_r = _rows(r, "r", self.n_embd)
@@ -234,8 +227,14 @@ class BlockNorm:
         elif out is not None and out[1] is not None:
             dtype = out[1].dtype
         nm = self.nm_ref if gate is None else C.byref(self.with_gate(gate, n, dtype, device))
-        self._weights_on(device)
-        ro, x, lro, ldx = self._outputs(r, dtype, out)
+        if self.device is not None and self.device != device:
+            raise ValueError(f"the norm's weights are on {self.device}, expected {device}")
+        if out is None:
+            h = lro = ldx = self.n_embd
+            ro = torch.empty(n, h, dtype=r.dtype, device=device)
+            x = torch.empty(n, h, dtype=dtype, device=device) if self.with_x else None
+        else:
+            ro, x, lro, ldx = self._check_out(r, dtype, out)
         rc = self.lib.moe_block_norm(nm, r.data_ptr(), DTYPES[r.dtype], ld_r, y_ptr, DTYPES[dtype], ld_y,
                                      None if ro is None else ro.data_ptr(), lro,
                                      None if x is None else x.data_ptr(), ldx, n, _raw_stream(index))
@@ -251,23 +250,31 @@ class BlockNorm:
             return _on_stream(lambda: self.combine(r, y_rows, pos, w, add, gate, out), stream,
                               (r, y_rows, pos, w, add, gate, self.post, self.pre) + (out or ()))
         index = r.get_device()
-        if index >= 0 and _elsewhere(index):
+        if index >= 0 and index != _current_device():
             with torch.cuda.device(index):
                 return self.combine(r, y_rows, pos, w, add, gate, out)
         f32 = (torch.float32,)
         h = self.n_embd
         ld_r, ld_rows = _rows(r, "r", h, f32), _rows(y_rows, "y_rows", h, f32)
         device, n = r.device, r.shape[0]
-        k = pos.shape[1] if pos.dim() == 2 else 0
-        if (k == 0 or pos.shape != (n, k) or w.shape != (n, k) or pos.dtype != torch.int32 or w.dtype != torch.float32
+        shape = pos.shape
+        k = shape[1] if len(shape) == 2 else 0
+        if (k == 0 or shape[0] != n or w.shape != shape or pos.dtype != torch.int32 or w.dtype != torch.float32
                 or not pos.is_contiguous() or not w.is_contiguous()):
             raise ValueError(f"pos and w must be contiguous int32 and fp32 [{n}, k]")
         if add is not None and (add.shape != (n, h) or add.dtype != torch.float32 or not add.is_contiguous()):
             raise ValueError(f"add must be a contiguous fp32 [{n}, {h}]")
-        _same_device(device, y_rows=y_rows, pos=pos, w=w, add=add)
+        if y_rows.device != device or pos.device != device or w.device != device or (add is not None and add.device != device):
+            raise ValueError(f"r is on {device}, and y_rows, pos, w and add must be")
         nm = self.nm_ref if gate is None else C.byref(self.with_gate(gate, n, torch.float32, device))
-        self._weights_on(device)
-        ro, x, lro, ldx = self._outputs(r, torch.float32, out)
+        if self.device is not None and self.device != device:
+            raise ValueError(f"the norm's weights are on {self.device}, expected {device}")
+        if out is None:
+            lro = ldx = h
+            ro = torch.empty(n, h, device=device, dtype=torch.float32)
+            x = torch.empty(n, h, device=device, dtype=torch.float32) if self.with_x else None
+        else:
+            ro, x, lro, ldx = self._check_out(r, torch.float32, out)
         rc = self.lib.moe_combine_norm(nm, r.data_ptr(), ld_r, y_rows.data_ptr(), ld_rows, y_rows.shape[0],
                                        pos.data_ptr(), w.data_ptr(), k, None if add is None else add.data_ptr(),
                                        None if ro is None else ro.data_ptr(), lro,
@@ -310,10 +317,11 @@ class AdapterSet:
             raise ValueError(f"rank {r} is above {self.MAX_RANK}")
         self.dtype, self.device = a.dtype, a.device
         pr, pc = -r % 8, -self.n_in % 8
-        self.a = a.new_zeros(self.n, r + pr, self.n_in + pc)
-        self.a[:, :r, :self.n_in] = a
-        self.b = b.new_zeros(self.n, self.n_out, r + pr)
-        self.b[:, :, :r] = b
+        # rank to a multiple of 8 and n_in to a multiple of 8, with zeros
+        self.a = torch.nn.functional.pad(a.detach(), (0, pc, 0, pr)) if pr or pc else a.detach().clone(
+            memory_format=torch.contiguous_format)
+        self.b = torch.nn.functional.pad(b.detach(), (0, pr)) if pr else b.detach().clone(
+            memory_format=torch.contiguous_format)
         if not isinstance(scale, torch.Tensor):
             scale = torch.full((self.n,), float(scale), device=self.device)
         elif scale.shape != (self.n,):
@@ -343,7 +351,7 @@ class AdapterSet:
             return _on_stream(lambda: self(x, ids, y, out, out_dtype), stream,
                               (x, ids, y, out, self.a, self.b, self.scale, self.rank))
         index = self.index
-        if _elsewhere(index):
+        if index != _current_device():
             with torch.cuda.device(index):
                 return self(x, ids, y, out, out_dtype)
         device = self.device

@@ -124,25 +124,25 @@ __device__ __forceinline__ void ad_add2(T *u, float v0, float v1, float f, bool 
         *reinterpret_cast<__nv_bfloat162 *>(u) = __floats2bfloat162_rn(a, b);
 }
 
-// 16 bytes of a row of n elements from element i on: asynchronous where the
-// row is aligned (vec), else element by element; zeros from n on and for a
-// null row.
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, int bytes) {   // zero-fills to 4
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// 16 bytes of an aligned row of n weights from i on; zeros from n on and for a
+// null row
 template <typename T>
-__device__ __forceinline__ void row16(uint8_t *dst, const T *row, int i, int n, bool vec) {
-    constexpr int E = 16 / (int)sizeof(T);
-    const int have = row ? min(max(n - i, 0), E) : 0;
-    if (have == 0) {
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    if (vec) {
-        cp16(smem_u32(dst), row + i, have * (int)sizeof(T));
-        return;
-    }
-    __align__(16) T v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = e < have ? row[i + e] : T(0.0f);
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(v);
+__device__ __forceinline__ void row16(uint8_t *dst, const T *row, int i, int n) {
+    const int have = row ? min(max(n - i, 0), 8) : 0;
+    if (have) cp16(smem_u32(dst), row + i, 2 * have);
+    else *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+}
+// one element of a row at any alignment (fp32 asynchronously); zero for have = false
+__device__ __forceinline__ void elem(uint8_t *dst, const float *src, bool have, const void *any) {
+    cp4(smem_u32(dst), have ? (const void *)src : any, have ? 4 : 0);
+}
+template <typename T>
+__device__ __forceinline__ void elem(uint8_t *dst, const T *src, bool have, const void *) {
+    *reinterpret_cast<T *>(dst) = have ? *src : T(0.0f);
 }
 
 }  // namespace
@@ -290,10 +290,10 @@ __device__ __forceinline__ void ad_copy_rows(const AdapterArgs &p, const int *s_
     }
 }
 
-// grid: tiles * cluster; M tokens per tile, up to 8 * NT ranks.  VEC: the rows of
-// x, y and out start at 16-byte boundaries.
-template <typename TX, typename TW, typename TO, int M, int NT, bool VEC>
-__global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(AdapterArgs p, AdSmem L) {
+// grid: tiles * cluster; M tokens per tile, up to 8 * NT ranks.  vec_x, vec_o: the
+// rows of x, and of y and out, start at 16-byte boundaries.
+template <typename TX, typename TW, typename TO, int M, int NT>
+__global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(AdapterArgs p, AdSmem L, int vec_x, int vec_o) {
     namespace cg = cooperative_groups;
     constexpr bool X16 = sizeof(TX) == 2;
     constexpr bool SCALED = std::is_same<TW, __half>::value;
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
     const int bp = ((p.rank + 15) & ~15) * 2 + 16;   // pitch of B and of the parts of A x
 
     // ---- loads: chunk k of x and A for the first product, chunk o of B and y for the second.
-    // A thread always loads the same 16-byte columns of the same rows, a whole
-    // chunk without a test per element.
+    // A whole chunk of aligned rows goes by 16 bytes, a thread always loading the same columns of the
+    // same rows; others go by elements, neighbouring threads taking neighbouring elements.
     constexpr int XE = 16 / (int)sizeof(TX), XC = KC / XE, XR = AD_THREADS / XC, XN = M / XR;   // x: XN rows per thread
     constexpr int AC = KC / 8, AR = AD_THREADS / AC, AN = (8 * NT + AR - 1) / AR;
     static_assert(M % XR == 0, "whole passes over the rows of x");
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
         const int xo = stage * (L.x_stage + L.a_stage) + tid / XC * XP + 16 * (tid % XC);
         const int ao = stage * (L.x_stage + L.a_stage) + L.x_stage + tid / AC * AP + 16 * (tid % AC);
         const int xc = k * KC + XE * (tid % XC), ac = k * KC + 8 * (tid % AC);
-        if (VEC && (k + 1) * KC <= p.n_in) {
+        if (vec_x && (k + 1) * KC <= p.n_in) {
 #pragma unroll
             for (int j = 0; j < XN; ++j)
                 cp16(sm0 + xo + j * XR * XP, (xrow[j] ? xrow[j] : (const TX *)p.x) + xc, xrow[j] ? 16 : 0);
@@ -352,12 +352,15 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
             }
             return;
         }
-#pragma unroll
-        for (int j = 0; j < XN; ++j) row16<TX>(sm + xo + j * XR * XP, xrow[j], xc, p.n_in, VEC);
+        for (int i = tid; i < M * KC; i += AD_THREADS) {
+            const int t = s_tok[i / KC], col = k * KC + i % KC;
+            elem(sm + stage * (L.x_stage + L.a_stage) + i / KC * XP + i % KC * (int)sizeof(TX),
+                 (const TX *)p.x + (int64_t)max(t, 0) * p.ld_x + col, t >= 0 && col < p.n_in, p.x);
+        }
 #pragma unroll
         for (int j = 0; j < AN; ++j) {
             const int r = tid / AC + j * AR;
-            if (r < r8) row16<TW>(sm + ao + j * AR * AP, r < rank ? A + (int64_t)r * p.lda : nullptr, ac, (int)p.lda, true);
+            if (r < r8) row16<TW>(sm + ao + j * AR * AP, r < rank ? A + (int64_t)r * p.lda : nullptr, ac, (int)p.lda);
         }
     };
     constexpr int BT = AD_THREADS / NC, BN = NT > BT ? NT / BT : 1;      // B: threads per row, 16-byte columns of each
@@ -378,26 +381,23 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
             if (8 * c >= r16) continue;
             const TW *src = B + (int64_t)row * p.rank;
             if (full && 8 * c + 8 <= rank) cp16(sm0 + bo + 16 * BT * j, src + 8 * c, 16);
-            else row16<TW>(sm + bo + 16 * BT * j, row < p.n_out ? src : nullptr, 8 * c, rank, true);
+            else row16<TW>(sm + bo + 16 * BT * j, row < p.n_out ? src : nullptr, 8 * c, rank);
         }
         if (!p.y) return;
+        if (vec_o && full) {
 #pragma unroll
-        for (int j = 0; j < YN; ++j) {
-            if (yt[j] < 0) continue;
-            const TO *src = (const TO *)p.y + (int64_t)yt[j] * p.ld_y;
-            if (VEC && full) cp16(sm0 + yo + j * YR * YP, src + yc, 16);
-            else row16<TO>(sm + yo + j * YR * YP, src, yc, p.n_out, VEC);
+            for (int j = 0; j < YN; ++j)
+                if (yt[j] >= 0) cp16(sm0 + yo + j * YR * YP, (const TO *)p.y + (int64_t)yt[j] * p.ld_y + yc, 16);
+            return;
+        }
+        for (int i = tid; i < cnt * NC; i += AD_THREADS) {
+            const int col = o * NC + i % NC;
+            if (col < p.n_out)
+                elem(sm + so + L.b_stage + i / NC * YP + i % NC * (int)sizeof(TO),
+                     (const TO *)p.y + (int64_t)s_tok[i / NC] * p.ld_y + col, true, p.y);
         }
     };
 
-    // y's tile comes into L2 while the first product runs
-    if (p.y) {
-        constexpr int LE = 128 / (int)sizeof(TO);
-        const int c0 = s0 * NC, lines = (min(s1 * NC, p.n_out) - c0 + LE - 1) / LE;
-        for (int i = warp; i < cnt; i += AD_WARPS)
-            for (int l = lane; l < lines; l += 32)
-                asm volatile("prefetch.global.L2 [%0];" ::"l"((const TO *)p.y + (int64_t)s_tok[i] * p.ld_y + c0 + l * LE));
-    }
     // ---- first product: this CTA's share of n_in, one MT x KW grid of warps
     const int kc = ((int)p.lda + KC - 1) / KC;
     const int k0 = (int)((int64_t)cr * kc / C), k1 = (int)((int64_t)(cr + 1) * kc / C);
@@ -566,6 +566,18 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
     const float f_lo = SCALED ? s_fac[m_lo] : 1.0f, f_hi = SCALED ? s_fac[m_lo + 8] : 1.0f;
     const uint32_t a_off = sm0 + (16 * mt + (lane & 15)) * bp + 16 * (lane >> 4);
     const uint32_t b_off = (8 * WN * kw + (lane & 7) + 8 * (lane >> 4)) * bp + 16 * (lane >> 3 & 1);
+    // the parts of A x are the same in every step: kept in registers up to rank 64
+    constexpr bool KEEP = NT <= 8;
+    constexpr int KS = KEEP ? NT / 2 : 1;
+    uint32_t keep[KS][P][4];
+    if (KEEP) {
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+            if (kk < r16 / 16) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) ldm4(keep[kk][i], a_off + i * M * bp + 32 * kk);
+            }
+    }
     stage = 0;
     for (int o = s0; o < s1; ++o) {
         if (L.b_stages == 3) cp_wait<1>();
@@ -578,17 +590,26 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
         float d[WN][4];
 #pragma unroll
         for (int n = 0; n < WN; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
-#pragma unroll 2
-        for (int kk = 0; kk < r16 / 16; ++kk) {
+        auto step = [&](int kk, const uint32_t (&af)[P][4]) {
             uint32_t bf[WN / 2][4];
 #pragma unroll
             for (int n = 0; n < WN; n += 2) ldm4(bf[n / 2], sm0 + so + b_off + 8 * n * bp + 32 * kk);
 #pragma unroll
-            for (int i = P - 1; i >= 0; --i) {   // the smallest parts first
-                uint32_t af[4];
-                ldm4(af, a_off + i * M * bp + 32 * kk);
+            for (int i = P - 1; i >= 0; --i)   // the smallest parts first
 #pragma unroll
-                for (int n = 0; n < WN; ++n) mma16(d[n], af, bf[n / 2][2 * (n & 1)], bf[n / 2][2 * (n & 1) + 1], TW());
+                for (int n = 0; n < WN; ++n) mma16(d[n], af[i], bf[n / 2][2 * (n & 1)], bf[n / 2][2 * (n & 1) + 1], TW());
+        };
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk)
+                if (kk < r16 / 16) step(kk, keep[kk]);
+        } else {
+#pragma unroll 2
+            for (int kk = 0; kk < r16 / 16; ++kk) {
+                uint32_t af[P][4];
+#pragma unroll
+                for (int i = 0; i < P; ++i) ldm4(af[i], a_off + i * M * bp + 32 * kk);
+                step(kk, af);
             }
         }
         TO *ys = reinterpret_cast<TO *>(sm + so + L.b_stage + m_lo * YP) + 8 * WN * kw + 2 * (lane & 3);
@@ -598,18 +619,20 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
             ad_add2(ys + 8 * n + 8 * YP / (int)sizeof(TO), d[n][2], d[n][3], f_hi, !p.y);
         }
         __syncthreads();
-        const int yc = o * NC + YE * (tid % YC);
-        const uint8_t *yo = sm + so + L.b_stage + tid / YC * YP + 16 * (tid % YC);
+        if (vec_o && (o + 1) * NC <= p.n_out) {
+            const uint8_t *yo = sm + so + L.b_stage + tid / YC * YP + 16 * (tid % YC);
 #pragma unroll
-        for (int j = 0; j < YN; ++j) {
-            if (yt[j] < 0 || yc >= p.n_out) continue;
-            TO *out = (TO *)p.out + (int64_t)yt[j] * p.ld_out + yc;
-            if (VEC && yc + YE <= p.n_out)
-                *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(yo + j * YR * YP);
-            else {
-                const TO *v = reinterpret_cast<const TO *>(yo + j * YR * YP);
-                for (int e = 0; e < YE && yc + e < p.n_out; ++e) out[e] = v[e];
-            }
+            for (int j = 0; j < YN; ++j)
+                if (yt[j] >= 0)
+                    *reinterpret_cast<uint4 *>((TO *)p.out + (int64_t)yt[j] * p.ld_out + o * NC + YE * (tid % YC)) =
+                        *reinterpret_cast<const uint4 *>(yo + j * YR * YP);
+            continue;
+        }
+        for (int i = tid; i < cnt * NC; i += AD_THREADS) {
+            const int col = o * NC + i % NC;
+            if (col < p.n_out)
+                ((TO *)p.out)[(int64_t)s_tok[i / NC] * p.ld_out + col] =
+                    *reinterpret_cast<const TO *>(sm + so + L.b_stage + i / NC * YP + i % NC * (int)sizeof(TO));
         }
     }
     cp_wait<0>();
@@ -649,10 +672,11 @@ static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
     auto al = [](const void *q, int64_t ld, int size) {
         return !q || (((uintptr_t)q | (uintptr_t)(ld * size)) & 15) == 0;
     };
-    const bool vec = al(p.x, p.ld_x, (int)sizeof(TX)) && al(p.y, p.ld_y, (int)sizeof(TO)) &&
-                     al(p.out, p.ld_out, (int)sizeof(TO));
-    auto *kern = vec ? k_adapters<TX, TW, TO, M, NT, true> : k_adapters<TX, TW, TO, M, NT, false>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L.bytes);
+    const int vec_x = al(p.x, p.ld_x, (int)sizeof(TX));
+    const int vec_o = al(p.y, p.ld_y, (int)sizeof(TO)) && al(p.out, p.ld_out, (int)sizeof(TO));
+    auto *kern = k_adapters<TX, TW, TO, M, NT>;
+    static SmemAttr attr;
+    cudaError_t e = attr.need((const void *)kern, L.bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles * C));
@@ -665,7 +689,7 @@ static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, p, L);
+    e = cudaLaunchKernelEx(&cfg, kern, p, L, vec_x, vec_o);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

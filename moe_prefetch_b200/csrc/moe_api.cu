@@ -1843,6 +1843,7 @@ extern "C" int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r
     if (ld_r < nm->n_embd || ld_rows < nm->n_embd || (r_out && ld_ro < nm->n_embd) || (x && ld_x < nm->n_embd))
         return fail(c, MOE_ERR_ARG, "moe_combine_norm: a row stride is below n_embd");
     if (r_out && r_out == x) return fail(c, MOE_ERR_ARG, "moe_combine_norm: r_out and x are the same");
+    if (y_rows && (r_out == y_rows || x == y_rows)) return fail(c, MOE_ERR_ARG, "moe_combine_norm: an output is y_rows");
     NormArgs a = norm_args(*nm, n_tok);
     a.r = r; a.ld_r = ld_r;
     a.y = y_rows; a.ld_y = ld_rows; a.n_rows = n_rows;
@@ -1889,6 +1890,7 @@ extern "C" int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, c
     if (!ids || !x || !out) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: a pointer is missing");
     if (ld_x < set->n_in || (y && ld_y < set->n_out) || ld_out < set->n_out)
         return fail(c, MOE_ERR_ARG, "moe_adapters_apply: a row stride is below the row");
+    if (out == x) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: out is x");
     if (y == out && ld_y != ld_out) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: y and out share memory with two strides");
     AdapterArgs p = adapter_args(*set, ids, n_tok);
     p.x = x; p.ld_x = ld_x;

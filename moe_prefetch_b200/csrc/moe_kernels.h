@@ -3,12 +3,31 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 
 #include "moe_dev.cuh"
 #include "moe_route.cuh"
 
 namespace moe {
+
+// cudaFuncSetAttribute of a kernel's dynamic shared memory, only where a launch on
+// this device needs more than any before (the call costs a microsecond).  One
+// object per kernel; launches may come from several threads.
+struct SmemAttr {
+    std::atomic<int> set[64];   // zero-initialised as a static
+    cudaError_t need(const void *fn, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 64 && set[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess || dev >= 64) return e;
+        int old = set[dev].load(std::memory_order_relaxed);
+        while (old < bytes && !set[dev].compare_exchange_weak(old, bytes, std::memory_order_release)) {}
+        return cudaSuccess;
+    }
+};
 
 // element types of the block operators (the MOE_DTYPE_* of include/moeb200.h)
 enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };

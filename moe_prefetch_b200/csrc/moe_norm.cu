@@ -370,9 +370,9 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     const size_t smem = (size_t)S * a.n_embd * (sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1));
     if (S) {
         per_sm = std::min(per_sm, (int)(220 * 1024 / (smem + 2048)));
+        static SmemAttr attr;
         if (smem > 40 * 1024 &&
-            (e = cudaFuncSetAttribute(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
+            (e = attr.need((const void *)k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>, (int)smem)) != cudaSuccess)
             return e;
     }
     per_sm = std::min(16, std::max(1, per_sm));

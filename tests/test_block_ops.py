@@ -60,14 +60,14 @@ def test_block_norm_refuses(kw, code):
 
 
 @pytest.mark.parametrize("kw,code", [(dict(k=0), ARG), (dict(pos=None), ARG), (dict(w=None), ARG), (dict(n_rows=-1), ARG),
-                                     (dict(ld_rows=63), ARG), (dict(rows=None), ARG)])
+                                     (dict(ld_rows=63), ARG), (dict(rows=None), ARG), (dict(r_out=C.c_void_p(5 << 20)), ARG)])
 def test_combine_norm_refuses(kw, code):
     from moe_prefetch_b200._lib import MoeNorm
-    d = dict(rows=PTR, ld_rows=64, n_rows=8, pos=PTR, w=PTR, k=2)
+    d = dict(rows=C.c_void_p(5 << 20), ld_rows=64, n_rows=8, pos=PTR, w=PTR, k=2, r_out=PTR)
     d.update(kw)
     nm = MoeNorm(64, 0, 0, 1.0, 1e-6, 0.0, None, None, None, 0)
     assert lib().moe_combine_norm(C.byref(nm), PTR, 64, d["rows"], d["ld_rows"], d["n_rows"], d["pos"], d["w"], d["k"],
-                                  None, PTR, 64, None, 64, 1, None) == code
+                                  None, d["r_out"], 64, None, 64, 1, None) == code
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -76,11 +76,11 @@ def test_combine_norm_refuses(kw, code):
     (dict(a=C.c_void_p(8)), ARG), (dict(scale=None), ARG), (dict(n_adapters=0), ARG), (dict(n_out=0), ARG),
     (dict(x_dtype=2), ARG), (dict(x_dtype=1, out_dtype=2), ARG), (dict(x_dtype=0, out_dtype=1), ARG),
     (dict(ids=None), ARG), (dict(x=None), ARG), (dict(ld_x=63), ARG), (dict(y=C.c_void_p(2 << 20), ld_y=31), ARG), (dict(ld_out=31), ARG),
-    (dict(y=PTR, out=PTR, ld_y=40), ARG), (dict(n_tok=-1), ARG)])
+    (dict(y=PTR, out=PTR, ld_y=40), ARG), (dict(x=C.c_void_p(3 << 20), out=C.c_void_p(3 << 20)), ARG), (dict(n_tok=-1), ARG)])
 def test_adapters_refuse(kw, code):
     from moe_prefetch_b200._lib import MoeAdapters
     d = dict(a=PTR, b=PTR, scale=PTR, ranks=None, n_adapters=2, rank=8, n_in=64, n_out=32, dtype=1, lda=64)
-    c = dict(ids=PTR, x=PTR, x_dtype=1, ld_x=64, y=None, ld_y=32, out=PTR, out_dtype=1, ld_out=32, n_tok=1)
+    c = dict(ids=PTR, x=C.c_void_p(4 << 20), x_dtype=1, ld_x=64, y=None, ld_y=32, out=PTR, out_dtype=1, ld_out=32, n_tok=1)
     for k, v in kw.items():
         (d if k in d else c)[k] = v
     if d["n_in"] > 64 and "ld_x" not in kw:

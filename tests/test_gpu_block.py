@@ -674,6 +674,68 @@ def test_block_layers_in_a_graph(stack):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_two_graphs_share_a_context(stack):
+    """Two captured layers of one context, of different sizes, replayed in
+    turn with eager calls between: the scratch they share holds nothing from
+    one call to the next."""
+    from moe_prefetch_b200 import AdapterSet, BlockNorm
+    nm = BlockNorm(H, post=1 + 0.2 * randn(H, seed=140), pre=1 + 0.2 * randn(H, seed=141))
+    ra = AdapterSet((randn(3, 8, H, seed=142) / 45).to(BF16), randn(3, stack.n_expert, 8, seed=143).to(BF16))
+    la = AdapterSet((randn(3, 8, H, seed=144) / 45).to(BF16), randn(3, H, 8, seed=145).to(BF16))
+    data, graphs = [], []
+    for n in (24, 5):      # the larger one first: it sizes the scratch
+        x, r = randn(n, H, seed=n), randn(n, H, seed=n + 1)
+        ids = torch.randint(-1, 3, (n,), generator=torch.Generator().manual_seed(n)).int().cuda()
+        call = lambda x=x, r=r, ids=ids: stack.block_forward(0, x, r=r, norm=nm, adapter_ids=ids, router_adapters=ra,
+                                                             adapters=la, path="gemv")
+        call()
+        data.append((x, call))
+    for x, call in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for turn in range(2):
+        for i, (x, call) in enumerate(data):
+            x.copy_(randn(*x.shape, seed=150 + 2 * turn + i))
+        for i in (1, 0, 1):
+            graphs[i][0].replay()
+            want = data[i][1]()
+            assert all(torch.equal(a, b) for a, b in zip(graphs[i][1], want))
+
+
+def test_calls_at_the_same_time():
+    """Two threads, each on its own stream, call the same objects."""
+    import threading
+    from moe_prefetch_b200 import AdapterSet, BlockNorm, Routing
+    rt = Routing(128, 8, score="sigmoid", bias=0.1 * randn(128, seed=1), n_group=4, topk_group=2, group_top=2)
+    nm = BlockNorm(512, post=1 + 0.2 * randn(512, seed=2), pre=True, gate_act="sigmoid")
+    st = AdapterSet((randn(4, 16, 512, seed=3) / 20).to(BF16), randn(4, 512, 16, seed=4).to(BF16))
+    work, bad = [], []
+    for i in range(2):
+        n = 40 + 500 * i
+        lg, r, y = randn(n, 128, seed=10 + i), randn(n, 512, seed=20 + i), randn(n, 512, seed=30 + i)
+        gate = randn(n, 1, seed=40 + i) if i else randn(n, 512, seed=40)
+        ids = torch.randint(-1, 4, (n,), generator=torch.Generator().manual_seed(i)).int().cuda()
+        work.append((lg, r, y, gate, ids, [*rt(lg), *nm(r, y, gate=gate), st(r, ids, y)]))
+    torch.cuda.synchronize()
+
+    def run(i):
+        lg, r, y, gate, ids, want = work[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = [*rt(lg), *nm(r, y, gate=gate), st(r, ids, y)]
+            torch.cuda.current_stream().synchronize()
+        if not all(torch.equal(a, b) for a, b in zip(got, want)):
+            bad.append(i)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_block_refusals(stack):
     from moe_prefetch_b200 import AdapterSet, BlockNorm, MoeError, Routing
     x = randn(4, H, seed=130)

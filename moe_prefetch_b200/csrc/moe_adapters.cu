@@ -645,9 +645,13 @@ static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
     const int kc = (int)((p.lda + KC - 1) / KC), oc = (p.n_out + NC - 1) / NC;
     // at most one partial tile per adapter in use (and for the rows without one)
     const int64_t tiles = std::min<int64_t>(p.n_tok, ((int64_t)p.n_tok + M - 1) / M + std::min(p.n_adapters + 1, p.n_tok));
-    // CTAs per tile: enough to fill the GPU, at most one per step of a product
+    // CTAs per tile: as many as one wave of two per SM holds (320: a few end early), at most one per
+    // step of a product.  The grid's bound counts a partial tile for every adapter; about three
+    // quarters of that is met.  512 / 2048 tokens, 8 adapters of rank 64, fp32: 8 CTAs 16.6 / 31.0
+    // us, 4 CTAs 18.6 / 35.1; 768 tokens: 8 CTAs 28.9 us, 4 CTAs 22.8.
+    const int64_t met = std::min<int64_t>(p.n_tok, p.n_tok / M + 1 + 3 * (int64_t)std::min(p.n_adapters + 1, p.n_tok) / 4);
     int C = 1;
-    while (C < 8 && tiles * C < 148 && 2 * C <= std::max(kc, oc)) C *= 2;
+    while (C < 8 && met * 2 * C <= 320 && 2 * C <= std::max(kc, oc)) C *= 2;
     AdSmem L{};
     L.x_stage = M * (KC * (int)sizeof(TX) + (sizeof(TX) == 2 ? 16 : 32));
     L.a_stage = p.rank * (KC * 2 + 16);
@@ -695,9 +699,14 @@ static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
 
 template <typename TX, typename TW, typename TO>
 static cudaError_t adapters_go(const AdapterArgs &p, cudaStream_t s) {
-    // tiles of 16 rows until there are enough rows to fill larger ones
-    if (p.n_tok <= 512)
-        return p.rank <= 32 ? adapters_launch<TX, TW, TO, 16, 4>(p, s) : adapters_launch<TX, TW, TO, 16, 16>(p, s);
+    // Tiles of 16 rows until there are enough rows to fill larger ones.  2048 -> 2048 columns, 8
+    // adapters in runs, rank 16 / 64 in bf16: 1024 tokens take 13.9 / 18.7 us with 16 rows and 14.6 /
+    // 20.6 us with 64, 2048 tokens 18.7 / 26.9 and 18.7 / 23.5 us, 4096 tokens 26.5 / 43.3 and 22.8 /
+    // 29.9 us.
+    if (p.n_tok <= 1536)
+        return p.rank <= 32   ? adapters_launch<TX, TW, TO, 16, 4>(p, s)
+               : p.rank <= 64 ? adapters_launch<TX, TW, TO, 16, 8>(p, s)
+                              : adapters_launch<TX, TW, TO, 16, 16>(p, s);
     return p.rank <= 64 ? adapters_launch<TX, TW, TO, 64, 8>(p, s) : adapters_launch<TX, TW, TO, 64, 16>(p, s);
 }
 

@@ -21,6 +21,7 @@ from ._lib import MoeAdapters, MoeNorm, MoeRouteCfg, check
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 SCORES = {"softmax": 0, "sigmoid": 1}
 ACTS = {"none": 0, "sigmoid": 1}
+_ROWS = torch.contiguous_format
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
 
 
@@ -230,9 +231,9 @@ class BlockNorm:
         if self.device is not None and self.device != device:
             raise ValueError(f"the norm's weights are on {self.device}, expected {device}")
         if out is None:
-            h = lro = ldx = self.n_embd
-            ro = torch.empty(n, h, dtype=r.dtype, device=device)
-            x = torch.empty(n, h, dtype=dtype, device=device) if self.with_x else None
+            lro = ldx = self.n_embd
+            ro = torch.empty_like(r, memory_format=_ROWS)
+            x = torch.empty_like(r if y is None else y, memory_format=_ROWS) if self.with_x else None
         else:
             ro, x, lro, ldx = self._check_out(r, dtype, out)
         rc = self.lib.moe_block_norm(nm, r.data_ptr(), DTYPES[r.dtype], ld_r, y_ptr, DTYPES[dtype], ld_y,
@@ -271,8 +272,8 @@ class BlockNorm:
             raise ValueError(f"the norm's weights are on {self.device}, expected {device}")
         if out is None:
             lro = ldx = h
-            ro = torch.empty(n, h, device=device, dtype=torch.float32)
-            x = torch.empty(n, h, device=device, dtype=torch.float32) if self.with_x else None
+            ro = torch.empty_like(r, memory_format=_ROWS)
+            x = torch.empty_like(r, memory_format=_ROWS) if self.with_x else None
         else:
             ro, x, lro, ldx = self._check_out(r, torch.float32, out)
         rc = self.lib.moe_combine_norm(nm, r.data_ptr(), ld_r, y_rows.data_ptr(), ld_rows, y_rows.shape[0],
@@ -368,7 +369,8 @@ class AdapterSet:
             if y.shape[0] != n or y.device != device:
                 raise ValueError(f"y has {y.shape[0]} rows on {y.device}, expected {n} on {device}")
         if out is None:
-            out = torch.empty(n, self.n_out, dtype=y.dtype if y is not None else out_dtype or x.dtype, device=device)
+            out = (torch.empty(n, self.n_out, dtype=out_dtype or x.dtype, device=device) if y is None
+                   else torch.empty_like(y, memory_format=_ROWS))
         else:
             ld_o = _rows(out, "out", self.n_out)
             if out.shape[0] != n or out.device != device or (y is not None and out.dtype != y.dtype):

@@ -71,16 +71,12 @@ __device__ __forceinline__ uint64_t route_key(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-__device__ __forceinline__ float route_val(uint32_t k) {   // the value of a 32-bit key
-    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
-}
-__device__ __forceinline__ float route_val(uint64_t) { return 0.0f; }   // (never asked)
-
-__device__ __forceinline__ uint32_t route_max(uint32_t v) { return __reduce_max_sync(MOE_FULL, v); }
-__device__ __forceinline__ uint64_t route_max(uint64_t v) {
-    const uint32_t hi = __reduce_max_sync(MOE_FULL, (uint32_t)(v >> 32));
-    const uint32_t lo = __reduce_max_sync(MOE_FULL, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
-    return (uint64_t)hi << 32 | lo;
+// Largest value of the warp, by shuffles: ptxas 12.9 miscompiles the integer
+// reduction of order-preserving keys turned back into a float.
+__device__ __forceinline__ float route_warp_max(float v) {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(MOE_FULL, v, off));
+    return v;
 }
 
 // The score of this lane's group: the largest clean value, or with group_top 2
@@ -125,32 +121,31 @@ __device__ __forceinline__ void route_cx(uint32_t &ka, int &ja, uint32_t &kb, in
     ja = j;
 }
 
+// Batcher's odd-even merge sort of a lane's J keys, largest first; cx(i, j) orders
+// entries i < j.
+template <int J, typename CX>
+__device__ __forceinline__ void route_sort(CX cx) {
+#pragma unroll
+    for (int p = 1; p < J; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j <= J - 1 - q; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < J && (i + j) / (2 * p) == (i + j + q) / (2 * p)) cx(i + j, i + j + q);
+}
+
 // The k largest keys (0: none) of the warp in order: returns rank r's expert in
-// lane r < k.  Up to eight keys per lane are sorted first (Batcher's odd-even
-// merge), so that a round looks at one key per lane; more are searched every
-// round.  With tol >= 0 the first k + 1 are compared, and -1 is returned when
-// two neighbours are within tol of each other: errors of tol / 2 could then
-// change the order.
+// lane r < k.  Up to eight keys per lane are sorted first, so that a round looks
+// at one key per lane; more are searched every round.
 template <int J>
-__device__ __forceinline__ int route_topk(uint32_t (&key)[J], const RouteSpec &s, const RouteLane &me, int lane,
-                                          float tol = -1.0f) {
+__device__ __forceinline__ int route_topk(uint32_t (&key)[J], const RouteSpec &s, const RouteLane &me, int lane) {
     constexpr bool SORT = J <= 8;
     int at[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) at[j] = j;
-    if constexpr (SORT) {
-#pragma unroll
-        for (int p = 1; p < J; p *= 2)
-#pragma unroll
-            for (int q = p; q >= 1; q /= 2)
-#pragma unroll
-                for (int j = q % p; j <= J - 1 - q; j += 2 * q)
-#pragma unroll
-                    for (int i = 0; i < q; ++i)
-                        if (i + j + q < J && (i + j) / (2 * p) == (i + j + q) / (2 * p))
-                            route_cx(key[i + j], at[i + j], key[i + j + q], at[i + j + q]);
-    }
-    float last = INFINITY;
+    if constexpr (SORT) route_sort<J>([&](int i, int j) { route_cx(key[i], at[i], key[j], at[j]); });
     int id_r = 0;
     for (int r = 0; r < s.k; ++r) {
         uint32_t best = key[0];
@@ -162,11 +157,6 @@ __device__ __forceinline__ int route_topk(uint32_t (&key)[J], const RouteSpec &s
         }
         const uint32_t m = __reduce_max_sync(MOE_FULL, best);
         const int id = (int)__reduce_min_sync(MOE_FULL, best == m ? (unsigned)me.expert(bj) : (unsigned)ROUTE_MAX_EXPERT);
-        if (tol >= 0.0f) {
-            const float v = route_val(m);
-            if (last - v <= tol) return -1;
-            last = v;
-        }
         const bool mine = best == m && me.expert(bj) == id;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -179,14 +169,45 @@ __device__ __forceinline__ int route_topk(uint32_t (&key)[J], const RouteSpec &s
         }
         if (lane == r) id_r = id;
     }
-    if (tol >= 0.0f) {   // and the best of those left out
+    return id_r;
+}
+
+// The same for keys that carry their place: value * 32 + (31 - j), so that a
+// comparison orders both at once and the sort is two instructions a pair.  The
+// first k + 1 are compared, and -1 is returned when two neighbours are within
+// tol of each other.
+template <int J>
+__device__ __forceinline__ int route_topk_packed(uint32_t (&key)[J], const RouteSpec &s, const RouteLane &me, int lane,
+                                                 uint32_t tol) {
+    constexpr bool SORT = J <= 8;
+    if constexpr (SORT)
+        route_sort<J>([&](int i, int j) {
+            const uint32_t hi = max(key[i], key[j]);
+            key[j] = min(key[i], key[j]);
+            key[i] = hi;
+        });
+    uint32_t last = 0xffffffffu;
+    int id_r = 0;
+    for (int r = 0; r <= s.k; ++r) {
         uint32_t best = key[0];
         if constexpr (!SORT) {
 #pragma unroll
             for (int j = 1; j < J; ++j) best = max(best, key[j]);
         }
-        best = __reduce_max_sync(MOE_FULL, best);
-        if (best && last - route_val(best) <= tol) return -1;
+        const uint32_t m = __reduce_max_sync(MOE_FULL, best);
+        if (r && m && last - m <= tol) return -1;   // (m = 0: no expert is left to be confused with)
+        if (r == s.k) break;
+        last = m;
+        // of lanes with the same key only one moves on: the next round then sees the tie
+        const int owner = __ffs(__ballot_sync(MOE_FULL, best == m)) - 1;
+        const bool mine = lane == owner;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if constexpr (SORT) key[j] = mine ? j + 1 < J ? key[j + 1 < J ? j + 1 : j] : 0u : key[j];
+            else key[j] = mine && key[j] == m ? 0u : key[j];
+        }
+        const int id = __shfl_sync(MOE_FULL, me.expert(31 - (int)(m & 31)), owner);
+        if (lane == r) id_r = id;
     }
     return id_r;
 }
@@ -219,22 +240,22 @@ __device__ __forceinline__ int route_topk(const double (&c)[J], uint32_t alive, 
 // 2^-24, the error of a value c is at most 10 u max(1, |c|) for sigmoid (expf 4 u
 // of a value below 1, a division of 4 u, two additions) and 30 u max(1, |c|) for
 // softmax (the sum's up to 15 additions, too): 2^-20 and 2^-18 are taken.  A
-// sum of two has twice that and its own rounding.
+// sum of two has twice that and its own rounding.  The values are then compared
+// as integers of 26 bits below the largest, with an error of 2^-26 more.
 template <int J>
 __device__ __forceinline__ int route_fast(const float (&l)[J], const RouteSpec &s, const RouteLane &me, float mx, int lane,
                                           float &total) {
-    float c[J], b[J], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, big = 1.0f;
-    bool ok = true;
+    float c[J], b[J], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, big = 1.0f, odd = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) b[j] = s.bias && j < me.count ? s.bias[me.expert(j)] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < J; ++j) c[j] = expf(s.sigmoid ? -l[j] : l[j] - mx);
+    for (int j = 0; j < J; ++j) c[j] = expf(s.sigmoid ? -l[j] : l[j] - mx);   // (a lane without a j-th expert: inf or 0)
     if (s.sigmoid) {
 #pragma unroll
         for (int j = 0; j < J; ++j) c[j] = __fdividef(1.0f, 1.0f + c[j]) + b[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < J; ++j) sum[j & 3] += j < me.count ? c[j] : 0.0f;
+        for (int j = 0; j < J; ++j) sum[j & 3] += c[j];
         total = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
         const float inv = 1.0f / total;
 #pragma unroll
@@ -242,26 +263,32 @@ __device__ __forceinline__ int route_fast(const float (&l)[J], const RouteSpec &
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const float v = j < me.count ? fabsf(c[j]) : 0.0f;
-        big = fmaxf(big, v);
-        ok = ok && v < INFINITY;
+        big = fmaxf(big, fabsf(c[j]));
+        odd = fmaf(c[j], 0.0f, odd);   // NaN once some value is not finite
     }
-    if (!__all_sync(MOE_FULL, ok)) return -1;
-    big = __uint_as_float(__reduce_max_sync(MOE_FULL, __float_as_uint(big)));   // (positive: ordered as integers)
+    if (!__all_sync(MOE_FULL, odd == 0.0f)) return -1;
+    big = route_warp_max(big);
     const float err = big * (s.sigmoid ? 0x1p-20f : 0x1p-18f);
     bool kept = true;
     if (s.n_group > 1) {
         const bool mine = me.group < s.n_group;
-        const uint32_t gk = route_key(route_group(c, me.count, s));
-        kept = route_group_kept(s, gk, me.group);
-        const uint32_t lo = __reduce_min_sync(MOE_FULL, mine && kept ? gk : 0xffffffffu);
-        const uint32_t hi = __reduce_max_sync(MOE_FULL, mine && !kept ? gk : 0u);
-        if (hi && route_val(lo) - route_val(hi) <= 6.0f * err) return -1;
+        const float g = route_group(c, me.count, s);
+        kept = route_group_kept(s, route_key(g), me.group);
+        const float lo = -route_warp_max(mine && kept ? -g : -INFINITY);   // the smallest kept
+        const float hi = route_warp_max(mine && !kept ? g : -INFINITY);    // the largest left out, if any
+        if (lo - hi <= 6.0f * err) return -1;
     }
+    // scaled by a power of two so that |c| <= 2^25
+    const uint32_t two = (__float_as_uint(big) + 0x7fffffu) & 0x7f800000u;   // big, rounded up to a power of two
+    if (two == 0x7f800000u) return -1;
+    const float scale = __uint_as_float(((127u + 25u + 127u) << 23) - two);
     uint32_t key[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) key[j] = kept && j < me.count ? route_key(c[j]) : 0u;
-    return route_topk(key, s, me, lane, 2.0f * err);
+    for (int j = 0; j < J; ++j) {
+        const int q = __float2int_rn(c[j] * scale) + (1 << 25) + 1;   // 1 .. 2^26 + 1
+        key[j] = kept && j < me.count ? (uint32_t)q * 32u + (31u - j) : 0u;
+    }
+    return route_topk_packed(key, s, me, lane, (uint32_t)__float2int_ru(2.0f * err * scale + 1.0f) * 32u + 31u);
 }
 
 // Selection by 64-bit values, which a softmax with a NaN or +inf logit (bad)
@@ -321,16 +348,21 @@ __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s,
     static_assert(J <= 32, "one bit of a mask per expert of a lane");
     const RouteLane me(s, lane);
     float l[J], mx = -INFINITY;
-    bool bad = false;
 #pragma unroll
     for (int j = 0; j < J; ++j) l[j] = j < me.count ? route_load(row + me.expert(j)) : -INFINITY;
+    if (!s.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        bad = bad || isnan(l[j]);
-        mx = fmaxf(mx, l[j]);
+        for (int j = 0; j < J; ++j) mx = fmaxf(mx, l[j]);
+        mx = route_warp_max(mx);
     }
-    mx = route_val(__reduce_max_sync(MOE_FULL, route_key(mx)));
-    bad = __any_sync(MOE_FULL, bad) || mx == INFINITY;   // then every softmax score is NaN
+    // a NaN, or for softmax +inf: then every softmax score is NaN
+    auto is_bad = [&]() {
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < J; ++j) bad = bad || isnan(l[j]);
+        return __any_sync(MOE_FULL, bad) || mx == INFINITY;
+    };
+    bool bad = false;
     float total = 0.0f;   // of e^(l - mx) over all experts
     if (!s.bias && !prior && (s.n_group == 1 || s.group_top == 1)) {
         uint32_t key[J];
@@ -344,10 +376,13 @@ __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s,
 #pragma unroll
         for (int j = 0; j < J; ++j) key[j] = kept && j < me.count ? route_key(route_clean(l[j])) : 0u;
         id_r = route_topk(key, s, me, lane);
+        bad = !s.sigmoid && is_bad();
     } else {
-        id_r = prior || bad ? -1 : route_fast<J>(l, s, me, mx, lane, total);
-        if (__any_sync(MOE_FULL, id_r < 0))
+        id_r = prior ? -1 : route_fast<J>(l, s, me, mx, lane, total);   // (no bad logits where it succeeds)
+        if (__any_sync(MOE_FULL, id_r < 0)) {
+            bad = is_bad();
             id_r = route_exact<J>(l, s, me, mx, bad, table, ns, delta, prior, pub, lane);
+        }
     }
     if (!s.sigmoid && !s.renorm) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};

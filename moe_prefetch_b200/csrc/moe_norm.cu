@@ -19,7 +19,7 @@
 
 namespace moe {
 
-// VEC values of one type as they are in memory: one by one (VEC 1), four (16
+// VEC values of one type as they are in memory: one by one (VEC 1), two, four (16
 // bytes of fp32, 8 of a 16-bit type) or eight of a 16-bit type.  A warp's
 // access then covers neighbouring whole sectors.
 template <typename T, int VEC> struct NormRaw;
@@ -28,6 +28,12 @@ template <typename T> struct NormRaw<T, 1> {
     __device__ __forceinline__ void load(const T *p) { u = *p; }
     __device__ __forceinline__ void zero() { u = T(0.0f); }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = (float)u; }
+};
+template <> struct NormRaw<float, 2> {
+    float2 a;
+    __device__ __forceinline__ void load(const float *p) { a = *reinterpret_cast<const float2 *>(p); }
+    __device__ __forceinline__ void zero() { a = make_float2(0.0f, 0.0f); }
+    __device__ __forceinline__ void get(float (&v)[2]) const { v[0] = a.x; v[1] = a.y; }
 };
 template <> struct NormRaw<float, 4> {
     float4 a;
@@ -46,15 +52,17 @@ template <> struct NormRaw<float, 8> {   // the norm weights beside 16-bit rows
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
 };
-template <typename T, int VEC> struct NormRaw {   // 16 bits, VEC 4 or 8
+template <typename T, int VEC> struct NormRaw {   // 16 bits, VEC 2, 4 or 8
     uint32_t u[VEC / 2];
     __device__ __forceinline__ void load(const T *p) {
         if constexpr (VEC == 8) {
             const uint4 a = *reinterpret_cast<const uint4 *>(p);
             u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
-        } else {
+        } else if constexpr (VEC == 4) {
             const uint2 a = *reinterpret_cast<const uint2 *>(p);
             u[0] = a.x; u[1] = a.y;
+        } else {
+            u[0] = *reinterpret_cast<const uint32_t *>(p);
         }
     }
     __device__ __forceinline__ void zero() {
@@ -92,6 +100,8 @@ __device__ __forceinline__ uint32_t norm_pack(float a, float b, __half) {
 template <typename T, int VEC>
 __device__ __forceinline__ void norm_store(T *p, const float (&v)[VEC]) {
     if constexpr (VEC == 1) *p = T(v[0]);
+    else if constexpr (VEC == 2 && std::is_same<T, float>::value) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+    else if constexpr (VEC == 2) *reinterpret_cast<uint32_t *>(p) = norm_pack(v[0], v[1], T());
     else if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
     else if constexpr (VEC == 4)
         *reinterpret_cast<uint2 *>(p) = make_uint2(norm_pack(v[0], v[1], T()), norm_pack(v[2], v[3], T()));
@@ -124,11 +134,18 @@ __device__ __forceinline__ float norm_sigmoid(float v) {
     return r;
 }
 
-// B bytes (8 or 16) into shared memory without a register.
+// B bytes (4, 8 or 16) into shared memory without a register.
 template <int B>
 __device__ __forceinline__ void norm_copy(void *dst, const void *src) {
     if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(B) : "memory");
+}
+
+// Bytes of a row in the ring: r, y, and the gate where it is full, each aligned to
+// its chunks (n_embd is a multiple of VEC), the row to 16.
+template <typename TR, typename TY>
+__host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
+    return (a.n_embd * (int)(sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1)) + 15) & ~15;
 }
 
 // A CTA takes rows blockIdx.x, + gridDim.x, ...; thread i holds the chunks of VEC
@@ -191,8 +208,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
             if (a.gate_kind == NORM_GATE_FULL) g_raw[c].load(gr + at(c));
         }
     };
-    // the ring: per row r, y, and the gate where it is full
-    const int row_bytes = H * (int)(sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1));
+    const int row_bytes = norm_row_bytes<TR, TY>(a);
     auto copy_row = [&](int64_t t, int stage) {
         uint8_t *dst = ring + stage * row_bytes;
 #pragma unroll
@@ -367,7 +383,7 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
     int per_sm = 1024 / threads;
-    const size_t smem = (size_t)S * a.n_embd * (sizeof(TR) + sizeof(TY) * (a.gate_kind == NORM_GATE_FULL ? 2 : 1));
+    const size_t smem = (size_t)S * norm_row_bytes<TR, TY>(a);
     if (S) {
         per_sm = std::min(per_sm, (int)(220 * 1024 / (smem + 2048)));
         static SmemAttr attr;
@@ -397,23 +413,27 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
 
 template <typename TR, typename TY>
 static cudaError_t norm_types(const NormArgs &a, cudaStream_t s) {
-    // 16-byte accesses need 8 values per chunk and aligned rows
-    auto al = [](const void *p, int64_t ld, size_t size) {
-        return !p || (((uintptr_t)p | (uintptr_t)(ld * (int64_t)size)) & 15) == 0;
+    // chunks of VEC values: as wide as the width divides and every row is aligned to
+    auto fits = [&](int vec) {
+        auto al = [&](const void *p, int64_t ld, size_t size) {
+            const uintptr_t m = std::min<uintptr_t>(16, vec * size) - 1;
+            return !p || (((uintptr_t)p | (uintptr_t)(ld * (int64_t)size)) & m) == 0;
+        };
+        return a.n_embd % vec == 0 && al(a.r, a.ld_r, sizeof(TR)) && al(a.r_out, a.ld_ro, sizeof(TR)) &&
+               al(a.y, a.ld_y, sizeof(TY)) && al(a.x, a.ld_x, sizeof(TY)) && al(a.add, a.n_embd, 4) && al(a.post, 0, 4) &&
+               al(a.pre, 0, 4) &&
+               (a.gate_kind == NORM_GATE_NONE || a.gate_kind == NORM_GATE_TOKEN ||
+                (a.gate_kind == NORM_GATE_FULL ? al(a.gate, a.ld_gate, sizeof(TY)) : al(a.gate, 0, 4)));
     };
     constexpr int VEC = std::is_same<TR, float>::value ? 4 : 8;
-    const bool vec = a.n_embd % 8 == 0 && al(a.r, a.ld_r, sizeof(TR)) && al(a.r_out, a.ld_ro, sizeof(TR)) &&
-                     al(a.y, a.ld_y, sizeof(TY)) && al(a.x, a.ld_x, sizeof(TY)) && al(a.add, a.n_embd, 4) &&
-                     al(a.post, 0, 4) && al(a.pre, 0, 4) &&
-                     (a.gate_kind == NORM_GATE_NONE || a.gate_kind == NORM_GATE_TOKEN ||
-                      al(a.gate, a.gate_kind == NORM_GATE_FULL ? a.ld_gate : 0, sizeof(TY)));
+    const int vec = fits(VEC) ? VEC : fits(2) ? 2 : 1;
     if (a.pos) {   // the expert rows of a layer are fp32
         if constexpr (std::is_same<TR, float>::value && std::is_same<TY, float>::value)
-            return vec ? norm_go<TR, TY, VEC, 1>(a, s) : norm_go<TR, TY, 1, 1>(a, s);
+            return vec == VEC ? norm_go<TR, TY, VEC, 1>(a, s) : vec == 2 ? norm_go<TR, TY, 2, 1>(a, s) : norm_go<TR, TY, 1, 1>(a, s);
         else
             return cudaErrorInvalidValue;
     }
-    return vec ? norm_go<TR, TY, VEC, 0>(a, s) : norm_go<TR, TY, 1, 0>(a, s);
+    return vec == VEC ? norm_go<TR, TY, VEC, 0>(a, s) : vec == 2 ? norm_go<TR, TY, 2, 0>(a, s) : norm_go<TR, TY, 1, 0>(a, s);
 }
 
 cudaError_t launch_block_norm(const NormArgs &a, int dt_r, int dt_y, cudaStream_t s) {

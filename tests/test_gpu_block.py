@@ -263,6 +263,15 @@ def test_norm_forms(gate, act, post, pre, off, h, pad):
     check_norm(6, h, F32, F32, post=post, gate=gate, act=act, pre=pre, off=off, pad=pad) if pre != "unit" else None
 
 
+@pytest.mark.parametrize("rt,yt", [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("h,pad", [(260, 0), (2052, 0), (254, 0), (2046, 2), (1022, 6), (1028, 4), (2050, 0), (6, 0), (12, 4)])
+def test_norm_chunk_widths(h, pad, rt, yt):
+    """Widths and row strides of every chunk size (8, 4, 2, 1 values), with
+    more rows than CTAs, so that the ring of rows turns."""
+    check_norm(1300, h, rt, yt, gate="full", act="sigmoid", pad=pad)
+    check_norm(3, h, rt, yt, gate="channel", pad=pad)
+
+
 @pytest.mark.parametrize("amp", [0.0, 1e-20, 1e18])
 def test_norm_extreme_rows(amp):
     """Zero rows, rows whose squares underflow, rows whose squares are large."""
@@ -292,7 +301,7 @@ def test_norm_first_block_and_partial_outputs():
             nm(r, **kw)
 
 
-@pytest.mark.parametrize("n,k,h", [(1, 8, 2048), (33, 9, 2048), (5, 1, 64), (4, 3, 1537), (2, 8, 16384)])
+@pytest.mark.parametrize("n,k,h", [(1, 8, 2048), (33, 9, 2048), (5, 1, 64), (4, 3, 1537), (3, 2, 1026), (2, 8, 16384)])
 @pytest.mark.parametrize("add", [False, True])
 def test_combine_norm(n, k, h, add):
     from moe_prefetch_b200 import BlockNorm

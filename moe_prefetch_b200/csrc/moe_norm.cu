@@ -155,14 +155,31 @@ __host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
 // memory, each thread copying and reading its own chunks (so the ring needs no
 // barrier): the kernel is bound by memory, and S - 1 rows are on their way while
 // one is in its two sums.
+// CTAs of 256 threads per SM: four, or three where the registers of a thread do
+// not fit (8,192 rows of 2,048 in bf16: 30.8 us with three and four rows in the
+// ring, 32.9 with four and three; fp32: 50.9 and 48.0; bf16 rows of 1,537: 73 and
+// 142).
+template <typename TR, int VEC, int SRC, int THREADS> constexpr int norm_ctas() {
+    return THREADS > 256 ? 1 : SRC == 0 && (VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
+}
+
 template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
-__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(NormArgs a) {
+__global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k_block_norm(NormArgs a) {
     static_assert(S == 0 || (SRC == 0 && VEC > 1), "the ring holds aligned rows");
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ __align__(16) float part[2][32];
     const int H = a.n_embd;
     const float inv_h = 1.0f / (float)H;   // each square is scaled first: the sum overflows only where the mean does
     auto at = [&](int c) { return VEC * ((int)threadIdx.x + c * (int)blockDim.x); };
+    bool in_[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) in_[c] = at(c) < H;
+    // whether the thread has chunk c: kept, or compared anew where registers are short (8,192 rows of
+    // 2,048 in fp32: 48.1 us against 50.9; of 4,096, with 512 threads: 45.7 against 44.6)
+    auto in = [&](int c) {
+        if constexpr (THREADS == 256 && VEC > 1) return at(c) < H;
+        else return in_[c];
+    };
     if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
     if (threadIdx.x + 32 < 64 && blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
     __syncthreads();
@@ -172,8 +189,8 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
         for (int c = 0; c < V; ++c) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) post[c][i] = pre[c][i] = 0.0f;
-            if (at(c) < H && a.post) norm_load(a.post + at(c), post[c]);
-            if (at(c) < H && a.pre) norm_load(a.pre + at(c), pre[c]);
+            if (in(c) && a.post) norm_load(a.post + at(c), post[c]);
+            if (in(c) && a.pre) norm_load(a.pre + at(c), pre[c]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 post[c][i] += a.offset;
@@ -202,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
         }
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            if (at(c) >= H) continue;
+            if (!in(c)) continue;
             r_raw[c].load((const TR *)a.r + t * a.ld_r + at(c));
             if (SRC == 0 && a.y) y_raw[c].load((const TY *)a.y + t * a.ld_y + at(c));
             if (a.gate_kind == NORM_GATE_FULL) g_raw[c].load(gr + at(c));
@@ -214,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             const int h = at(c);
-            if (h >= H) continue;
+            if (!in(c)) continue;
             norm_copy<VEC * (int)sizeof(TR)>(dst + h * (int)sizeof(TR), (const TR *)a.r + t * a.ld_r + h);
             uint8_t *dy = dst + H * (int)sizeof(TR) + h * (int)sizeof(TY);
             if (a.y) norm_copy<VEC * (int)sizeof(TY)>(dy, (const TY *)a.y + t * a.ld_y + h);
@@ -232,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             const int h = at(c);
-            if (h >= H) continue;
+            if (!in(c)) continue;
             r_raw[c].load((const TR *)src + h);
             const TY *sy = (const TY *)(src + H * (int)sizeof(TR)) + h;
             if (a.y) y_raw[c].load(sy);
@@ -283,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
                     for (int c = 0; c < V; ++c) {
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) v[u][c][i] = 0.0f;
-                        if (at(c) < H && q >= 0 && q < a.n_rows) norm_load(rows + (int64_t)q * a.ld_y + at(c), v[u][c]);
+                        if (in(c) && q >= 0 && q < a.n_rows) norm_load(rows + (int64_t)q * a.ld_y + at(c), v[u][c]);
                     }
                 }
 #pragma unroll
@@ -299,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
             if (a.add) {
 #pragma unroll
                 for (int c = 0; c < V; ++c)
-                    if (at(c) < H) {
+                    if (in(c)) {
                         float v[VEC];
                         norm_load(a.add + t * H + at(c), v);
 #pragma unroll
@@ -317,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
         } else if (a.gate_kind != NORM_GATE_NONE) {
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                if (a.gate_kind == NORM_GATE_CHANNEL && at(c) < H) norm_load((const float *)a.gate + at(c), f[c]);
+                if (a.gate_kind == NORM_GATE_CHANNEL && in(c)) norm_load((const float *)a.gate + at(c), f[c]);
                 if (a.sigmoid) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
@@ -348,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
         TR *ro = (TR *)a.r_out + t * a.ld_ro;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            if (at(c) >= H) continue;   // (r is 0 there and adds nothing)
+            if (!in(c)) continue;       // (r is 0 there and adds nothing)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 r[c][i] = a.post || a.gate_kind != NORM_GATE_NONE ? fmaf(y[c][i] * by, f[c][i], r[c][i])
@@ -365,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 4) k_block_norm(N
         TY *xo = (TY *)a.x + t * a.ld_x;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            if (at(c) >= H) continue;
+            if (!in(c)) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) r[c][i] *= inv * pre[c][i];
             norm_store(xo + at(c), r[c]);
@@ -382,7 +399,7 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     cudaError_t e;
     if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    int per_sm = 1024 / threads;
+    int per_sm = (THREADS > 256 ? 1024 : 256 * norm_ctas<TR, VEC, SRC, THREADS>()) / threads;
     const size_t smem = (size_t)S * norm_row_bytes<TR, TY>(a);
     if (S) {
         per_sm = std::min(per_sm, (int)(220 * 1024 / (smem + 2048)));
@@ -405,10 +422,10 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const bool wide = chunks > 1024 * V8;
     const int per = wide ? 2 * V8 : V8;
     const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;
-    constexpr bool RING = VEC > 1 && SRC == 0;   // up to 12 bytes a value: 3 rows of 2048, 2 of 8192
+    constexpr bool RING = VEC > 1 && SRC == 0;   // up to 12 bytes a value: 3 rows of 2048 (4 of 16 bits), 2 of 8192
     if (wide) return norm_launch<TR, TY, VEC, 2 * V8, SRC, 1024, 0>(a, threads, s);
     return threads > 256 ? norm_launch<TR, TY, VEC, V8, SRC, 1024, RING ? 2 : 0>(a, threads, s)
-                         : norm_launch<TR, TY, VEC, V8, SRC, 256, RING ? 3 : 0>(a, threads, s);
+                         : norm_launch<TR, TY, VEC, V8, SRC, 256, !RING ? 0 : sizeof(TR) == 2 ? 4 : 3>(a, threads, s);
 }
 
 template <typename TR, typename TY>

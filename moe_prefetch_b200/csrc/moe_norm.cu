@@ -157,7 +157,7 @@ __host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
 // one is in its two sums.
 // CTAs of 256 threads per SM: four, or three where the registers of a thread do
 // not fit (8,192 rows of 2,048 in bf16: 30.8 us with three and four rows in the
-// ring, 32.9 with four and three; fp32: 50.9 and 48.0; bf16 rows of 1,537: 73 and
+// ring, 32.9 with four and three; fp32: 50.9 and 48.0; bf16 rows of 1,537: 84 and
 // 142).
 template <typename TR, int VEC, int SRC, int THREADS> constexpr int norm_ctas() {
     return THREADS > 256 ? 1 : SRC == 0 && (VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
@@ -391,6 +391,142 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
     }
 }
 
+// Rows wider than 8192, or wider than 2048 and of an odd width or alignment (VEC
+// 1): a CTA per row keeps it in shared memory as fp32 (y, then r'), and each of
+// the three passes has U chunks per thread in flight.  With a row in the registers
+// of one CTA too few threads fit an SM: 2,046 rows of 8,200 in fp32 take 64 us
+// (114 in registers), 3,928 of 4,271 in bf16 114 us (210); 10,915 of 1,537 would
+// take 106 (84).
+template <typename TR, typename TY, int VEC, int SRC>
+__global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
+    extern __shared__ __align__(16) float row[];   // [n_embd]
+    __shared__ __align__(16) float part[2][32];
+    constexpr int U = VEC == 1 ? 8 : VEC == 2 ? 4 : VEC == 4 ? 2 : 1;
+    const int H = a.n_embd, step = VEC * (int)blockDim.x, h0 = VEC * (int)threadIdx.x;
+    const float inv_h = 1.0f / (float)H;
+    const int64_t t = blockIdx.x;
+    if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
+    if (blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
+    __syncthreads();
+    const bool y_first = SRC == 1 || a.post;       // y is needed whole before r'
+    float by = a.scale;
+    if (y_first) {
+        float ss = 0.0f;
+        for (int b = h0; b < H; b += U * step) {
+            float y[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) y[u][i] = 0.0f;
+                if (SRC == 0 && b + u * step < H) norm_load((const TY *)a.y + t * a.ld_y + b + u * step, y[u]);
+            }
+            if (SRC == 1) {   // the chain of k_combine: fma from 0 in rank order, then + add
+                for (int j = 0; j < a.k; ++j) {
+                    const int q = a.pos[t * a.k + j];
+                    const float w = a.w[t * a.k + j];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        float v[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
+                        if (b + u * step < H && q >= 0 && q < a.n_rows)
+                            norm_load((const float *)a.y + (int64_t)q * a.ld_y + b + u * step, v);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) y[u][i] = __fmaf_rn(w, v[i], y[u][i]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (a.add && b + u * step < H) {
+                        float v[VEC];
+                        norm_load(a.add + t * H + b + u * step, v);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) y[u][i] = __fadd_rn(y[u][i], v[i]);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (b + u * step < H) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        row[b + u * step + i] = y[u][i];
+                        ss = fmaf(y[u][i] * inv_h, y[u][i], ss);
+                    }
+                }
+        }
+        if (a.post) by *= rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
+    }
+    float g_tok = 1.0f;
+    if (a.gate_kind == NORM_GATE_TOKEN) {
+        float v[1];
+        norm_load((const TY *)a.gate + t * a.ld_gate, v);
+        g_tok = a.sigmoid ? norm_sigmoid(v[0]) : v[0];
+    }
+    const bool each = a.gate_kind == NORM_GATE_FULL || a.gate_kind == NORM_GATE_CHANNEL;
+    float ss = 0.0f;
+    for (int b = h0; b < H; b += U * step) {
+        NormRaw<TR, VEC> r[U];
+        NormRaw<TY, VEC> y[U], g[U];
+        NormRaw<float, VEC> gc[U], po[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = b + u * step;
+            if (h >= H) continue;
+            r[u].load((const TR *)a.r + t * a.ld_r + h);
+            if (!y_first && a.y) y[u].load((const TY *)a.y + t * a.ld_y + h);
+            if (a.gate_kind == NORM_GATE_FULL) g[u].load((const TY *)a.gate + t * a.ld_gate + h);
+            else if (each) gc[u].load((const float *)a.gate + h);
+            if (a.post) po[u].load(a.post + h);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = b + u * step;
+            if (h >= H) continue;
+            float rv[VEC], yv[VEC], f[VEC], p[VEC];
+            r[u].get(rv);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                f[i] = g_tok;
+                p[i] = 1.0f - a.offset;
+                yv[i] = y_first ? row[h + i] : 0.0f;
+            }
+            if (!y_first && a.y) y[u].get(yv);
+            if (a.gate_kind == NORM_GATE_FULL) g[u].get(f);
+            else if (each) gc[u].get(f);
+            if (a.post) po[u].get(p);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if (each && a.sigmoid) f[i] = norm_sigmoid(f[i]);
+                if (a.post) f[i] *= p[i] + a.offset;
+                rv[i] = fmaf(yv[i] * by, f[i], rv[i]);
+                ss = fmaf(rv[i] * inv_h, rv[i], ss);
+                row[h + i] = rv[i];
+            }
+            if (a.r_out) norm_store((TR *)a.r_out + t * a.ld_ro + h, rv);
+        }
+    }
+    if (!a.x) return;
+    const float inv = rsqrtf(norm_cta_sum(ss, part[1]) + a.eps);
+    for (int b = h0; b < H; b += U * step) {
+        NormRaw<float, VEC> pr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (a.pre && b + u * step < H) pr[u].load(a.pre + b + u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = b + u * step;
+            if (h >= H) continue;
+            float p[VEC], v[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) p[i] = 1.0f - a.offset;
+            if (a.pre) pr[u].get(p);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = row[h + i] * (a.pre ? inv * (p[i] + a.offset) : inv);
+            norm_store((TY *)a.x + t * a.ld_x + h, v);
+        }
+    }
+}
+
 template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
 static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     // as many CTAs as the GPU holds, at most one per row; the combine takes a CTA
@@ -417,15 +553,22 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
 template <typename TR, typename TY, int VEC, int SRC>
 static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const int chunks = (a.n_embd + VEC - 1) / VEC;
-    // 8 values per thread where a CTA holds the row that way, else 16
-    constexpr int V8 = 8 / VEC;
-    const bool wide = chunks > 1024 * V8;
-    const int per = wide ? 2 * V8 : V8;
-    const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;
-    constexpr bool RING = VEC > 1 && SRC == 0;   // up to 12 bytes a value: 3 rows of 2048 (4 of 16 bits), 2 of 8192
-    if (wide) return norm_launch<TR, TY, VEC, 2 * V8, SRC, 1024, 0>(a, threads, s);
-    return threads > 256 ? norm_launch<TR, TY, VEC, V8, SRC, 1024, RING ? 2 : 0>(a, threads, s)
-                         : norm_launch<TR, TY, VEC, V8, SRC, 256, !RING ? 0 : sizeof(TR) == 2 ? 4 : 3>(a, threads, s);
+    if (a.n_embd > (VEC == 1 ? 2048 : 8192)) {
+        const size_t smem = sizeof(float) * (size_t)a.n_embd;
+        static SmemAttr attr;
+        cudaError_t e;
+        if (smem > 40 * 1024 && (e = attr.need((const void *)k_block_norm_wide<TR, TY, VEC, SRC>, (int)smem)) != cudaSuccess)
+            return e;
+        const int threads = std::min(256, (chunks + 255) / 256 * 32);   // eight chunks a thread while there are few
+        k_block_norm_wide<TR, TY, VEC, SRC><<<a.n_tok, threads, smem, s>>>(a);
+        return cudaGetLastError();
+    }
+    constexpr int V = 8 / VEC;                      // 8 values per thread
+    constexpr bool RING = VEC > 1 && SRC == 0;      // up to 12 bytes a value: 3 rows of 2048 (4 of 16 bits), 2 of 8192
+    const int threads = ((chunks + V - 1) / V + 31) / 32 * 32;
+    if constexpr (VEC > 1)
+        if (threads > 256) return norm_launch<TR, TY, VEC, V, SRC, 1024, RING ? 2 : 0>(a, threads, s);
+    return norm_launch<TR, TY, VEC, V, SRC, 256, !RING ? 0 : sizeof(TR) == 2 ? 4 : 3>(a, threads, s);
 }
 
 template <typename TR, typename TY>

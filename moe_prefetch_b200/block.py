@@ -66,6 +66,9 @@ def _same_device(device, **tensors):
 def _on_stream(call, stream, tensors):
     """call() with `stream` current, which its device's allocator then knows
     the tensors are used on."""
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device != stream.device:
+            raise ValueError(f"the stream is on {stream.device}, a tensor on {t.device}")
     with torch.cuda.stream(stream):
         out = call()
     for t in tensors:
@@ -86,7 +89,9 @@ class Routing:
     divided by their sum (renorm) and multiplied by scale.
 
     ``routing(logits)`` -> ids int32 [n, k], w fp32 [n, k].  Ties go to the
-    lower expert; -inf logits mark experts that a token may not use."""
+    lower expert; a logit of -inf has score 0, and with a bias of -inf an expert
+    is chosen last.  The bias tensor is read at every call, so that a change of
+    its values is seen (MoeStack.set_routing copies it)."""
 
     def __init__(self, n_expert, k, score="softmax", bias=None, n_group=1, topk_group=None, group_top=1,
                  renorm=True, scale=1.0):
@@ -303,6 +308,8 @@ class AdapterSet:
             if not a or len(a) != len(b) or rank is not None:
                 raise ValueError("lists of adapters: one a and one b each, and no rank")
             ranks = [t.shape[0] for t in a]
+            if [t.shape[-1] for t in b] != ranks:
+                raise ValueError(f"ranks {ranks} of a, {[t.shape[-1] for t in b]} of b")
             a = torch.stack([torch.nn.functional.pad(t, (0, 0, 0, max(ranks) - t.shape[0])) for t in a])
             b = torch.stack([torch.nn.functional.pad(t, (0, max(ranks) - t.shape[1])) for t in b])
             rank = torch.tensor(ranks, dtype=torch.int32, device=a.device)

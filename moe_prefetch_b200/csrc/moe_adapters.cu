@@ -97,7 +97,6 @@ __device__ __forceinline__ void pair32(uint32_t u, uint32_t &b0, uint32_t &b1, _
     b1 = __float_as_uint(f.y);
 }
 
-
 __device__ __forceinline__ uint2 ad_pack(const float (&v)[4], __nv_bfloat16) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
     return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
@@ -710,8 +709,7 @@ static cudaError_t adapters_go(const AdapterArgs &p, cudaStream_t s) {
     return p.rank <= 64 ? adapters_launch<TX, TW, TO, 64, 8>(p, s) : adapters_launch<TX, TW, TO, 64, 16>(p, s);
 }
 
-cudaError_t launch_adapters(const AdapterArgs &p, int dt_x, int dt_w, int dt_out, cudaStream_t s) {
-    if (p.n_tok == 0) return cudaSuccess;
+static cudaError_t adapters_chunk(const AdapterArgs &p, int dt_x, int dt_w, int dt_out, cudaStream_t s) {
     if (dt_x == DT_F32 && dt_out == DT_F32)
         return dt_w == DT_BF16 ? adapters_go<float, __nv_bfloat16, float>(p, s) : adapters_go<float, __half, float>(p, s);
     if (dt_x != dt_w || (dt_out != dt_w && dt_out != DT_F32)) return cudaErrorInvalidValue;
@@ -719,6 +717,24 @@ cudaError_t launch_adapters(const AdapterArgs &p, int dt_x, int dt_w, int dt_out
         return dt_out == DT_F32 ? adapters_go<__nv_bfloat16, __nv_bfloat16, float>(p, s)
                                 : adapters_go<__nv_bfloat16, __nv_bfloat16, __nv_bfloat16>(p, s);
     return dt_out == DT_F32 ? adapters_go<__half, __half, float>(p, s) : adapters_go<__half, __half, __half>(p, s);
+}
+
+cudaError_t launch_adapters(const AdapterArgs &p, int dt_x, int dt_w, int dt_out, cudaStream_t s) {
+    // Every CTA reads all ids of its launch to find its tile, so a launch takes up to 8192 tokens: about
+    // one wave of two CTAs per SM, and the ids stay a small part of what a CTA reads.
+    constexpr int CHUNK = 8192;
+    const int64_t sx = dt_x == DT_F32 ? 4 : 2, so = dt_out == DT_F32 ? 4 : 2;
+    for (int64_t t = 0; t < p.n_tok; t += CHUNK) {
+        AdapterArgs c = p;
+        c.n_tok = (int)std::min<int64_t>(CHUNK, p.n_tok - t);
+        c.ids = p.ids + t;
+        c.x = (const uint8_t *)p.x + t * p.ld_x * sx;
+        c.y = p.y ? (const uint8_t *)p.y + t * p.ld_y * so : nullptr;
+        c.out = (uint8_t *)p.out + t * p.ld_out * so;
+        const cudaError_t e = adapters_chunk(c, dt_x, dt_w, dt_out, s);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace moe

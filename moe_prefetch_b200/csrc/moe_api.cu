@@ -1979,7 +1979,7 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
         p.out = y ? y : delta; p.ld_out = H;
         CK(launch_adapters(p, DT_F32, la->dtype, DT_F32, s));
     }
-    // the lookahead of a streaming context reads x, which x_out may overwrite
+    // the lookahead of a streaming context reads x, which the outputs may overwrite
     if (b->norm) {
         NormArgs a = norm_args(*b->norm, n_tok);
         a.r = b->r; a.ld_r = H;
@@ -1987,7 +1987,7 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
         a.pos = c->grp.pair_pos; a.w = w_e; a.k = kx; a.add = delta;
         a.r_out = b->r_out; a.ld_ro = H;
         a.x = b->x_out; a.ld_x = H;
-        const bool ahead = n_tok == 1 && g.stream && b->x_out == x;
+        const bool ahead = n_tok == 1 && g.stream && (b->x_out == x || b->r_out == x);
         if (ahead && (rc = after_observe(c, layer, ids_d, g.n_used, s, x)) != MOE_OK) return rc;
         CK(launch_block_norm(a, DT_F32, DT_F32, s));
         if (ahead) return MOE_OK;

@@ -433,6 +433,22 @@ def test_adapters_long(n, n_in, n_out, na, r, order, xt, wt, ot):
     check_adapters(n, n_in, n_out, na, r, xt, wt, ot, order=order, ragged=na < 10)
 
 
+def test_adapters_more_tokens_than_a_launch():
+    """A call of more tokens than one launch takes, in place, against the same
+    rows in two calls."""
+    from moe_prefetch_b200 import AdapterSet
+    st = AdapterSet((randn(3, 8, 40, seed=1) / 6).to(BF16), randn(3, 24, 8, seed=2).to(BF16), scale=0.5)
+    n, cut = 20001, 8192
+    x, y = randn(n, 40, seed=3), randn(n, 24, seed=4)
+    ids = torch.randint(-1, 3, (n,), generator=torch.Generator().manual_seed(5)).int().cuda()
+    want = torch.cat([st(x[a:b], ids[a:b].clone(), y[a:b]) for a, b in ((0, cut), (cut, 2 * cut), (2 * cut, n))])
+    assert torch.equal(st(x, ids, y), want)
+    ref, bound = adapters_ref(x[-50:], y[-50:], st.a[:, :, :40], st.b, st.scale, None, ids[-50:])
+    close(want[-50:], ref, bound, "out")
+    st(x, ids, y, out=y)
+    assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize("xt,wt,ot", TYPES)
 @pytest.mark.parametrize("n", [7, 600])
 def test_adapters_extreme_values(n, xt, wt, ot):
@@ -471,6 +487,8 @@ def test_adapters_lists_empty_refusals():
                  lambda: st(x, ids.cpu()), lambda: st(x.cpu(), ids)):
         with pytest.raises(ValueError):
             call()
+    with pytest.raises(ValueError):    # an a and a b of different ranks
+        AdapterSet(a, b[::-1])
     from moe_prefetch_b200 import MoeError
     with pytest.raises(MoeError):      # fp16 rows beside bf16 weights
         st(x.half(), ids)

@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
     const int C = (int)cl.num_blocks(), cr = (int)cl.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int a, cnt;
+    pdl_enter();
     if (!ad_find_tile<M>(p, blockIdx.x / C, reinterpret_cast<int *>(sm + L.off_hist), s_tok, a, cnt)) return;
     const int oc = (p.n_out + NC - 1) / NC;                  // output steps, this CTA's [s0, s1)
     const int s0 = (int)((int64_t)cr * oc / C), s1 = (int)((int64_t)(cr + 1) * oc / C);
@@ -679,21 +680,9 @@ static cudaError_t adapters_launch(const AdapterArgs &p, cudaStream_t s) {
     const int vec_o = al(p.y, p.ld_y, (int)sizeof(TO)) && al(p.out, p.ld_out, (int)sizeof(TO));
     auto *kern = k_adapters<TX, TW, TO, M, NT>;
     static SmemAttr attr;
-    cudaError_t e = attr.need((const void *)kern, L.bytes);
+    const cudaError_t e = attr.need((const void *)kern, L.bytes);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * C));
-    cfg.blockDim = dim3(AD_THREADS);
-    cfg.dynamicSmemBytes = L.bytes;
-    cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = C;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, p, L, vec_x, vec_o);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return launch_pdl(kern, (unsigned)(tiles * C), AD_THREADS, L.bytes, s, C, p, L, vec_x, vec_o);
 }
 
 template <typename TX, typename TW, typename TO>

@@ -1215,6 +1215,14 @@ __device__ __forceinline__ float warp_sum4_t(float a, float b, float c, float d,
 // bulk copies, mbarriers, timers
 // ---------------------------------------------------------------------------
 
+// The start of a kernel launched by launch_pdl, before its first access to
+// global memory: waits until the kernels before it have ended and their writes
+// are visible, then lets the next such kernel take its places.
+__device__ __forceinline__ void pdl_enter() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }

@@ -29,6 +29,29 @@ struct SmemAttr {
     }
 };
 
+// Launch a kernel that starts with pdl_enter(): its CTAs may take their places while
+// the kernel before it on the stream is still in its last wave, and wait there
+// for its end (programmatic stream serialisation), which hides the launch.
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kern)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, int cluster,
+                       A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, P(args)...);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 // element types of the block operators (the MOE_DTYPE_* of include/moeb200.h)
 enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 

@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
     if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
     if (threadIdx.x + 32 < 64 && blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
     __syncthreads();
+    pdl_enter();
     float post[V][VEC], pre[V][VEC];        // weight + offset
     auto load_weights = [&]() {
 #pragma unroll
@@ -408,6 +409,7 @@ __global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
     if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
     if (blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
     __syncthreads();
+    pdl_enter();
     const bool y_first = SRC == 1 || a.post;       // y is needed whole before r'
     float by = a.scale;
     if (y_first) {
@@ -545,9 +547,8 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
             return e;
     }
     per_sm = std::min(16, std::max(1, per_sm));
-    k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>
-        <<<SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads, smem, s>>>(a);
-    return cudaGetLastError();
+    return launch_pdl(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>, SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads,
+                      smem, s, 0, a);
 }
 
 template <typename TR, typename TY, int VEC, int SRC>
@@ -560,8 +561,7 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
         if (smem > 40 * 1024 && (e = attr.need((const void *)k_block_norm_wide<TR, TY, VEC, SRC>, (int)smem)) != cudaSuccess)
             return e;
         const int threads = std::min(256, (chunks + 255) / 256 * 32);   // eight chunks a thread while there are few
-        k_block_norm_wide<TR, TY, VEC, SRC><<<a.n_tok, threads, smem, s>>>(a);
-        return cudaGetLastError();
+        return launch_pdl(k_block_norm_wide<TR, TY, VEC, SRC>, a.n_tok, threads, smem, s, 0, a);
     }
     constexpr int V = 8 / VEC;                      // 8 values per thread
     constexpr bool RING = VEC > 1 && SRC == 0;      // up to 12 bytes a value: 3 rows of 2048 (4 of 16 bits), 2 of 8192

@@ -10,6 +10,7 @@ template <typename T, int J>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
     k_route(RouteSpec spec, const T *__restrict__ logits, int64_t ld, int n_tok, int32_t *__restrict__ ids,
             float *__restrict__ w) {
+    pdl_enter();
     const int lane = threadIdx.x & 31;
     const int t = blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
     if (t >= n_tok) return;
@@ -46,12 +47,11 @@ static cudaError_t route_j(const RouteSpec &sp, const T *logits, int64_t ld, int
                            cudaStream_t s) {
     const int grid = (n_tok - 1) / ROUTE_WARPS + 1;
     const int j = route_per_lane(sp);
-    if (j <= 2) k_route<T, 2><<<grid, ROUTE_WARPS * 32, 0, s>>>(sp, logits, ld, n_tok, ids, w);
-    else if (j <= 4) k_route<T, 4><<<grid, ROUTE_WARPS * 32, 0, s>>>(sp, logits, ld, n_tok, ids, w);
-    else if (j <= 8) k_route<T, 8><<<grid, ROUTE_WARPS * 32, 0, s>>>(sp, logits, ld, n_tok, ids, w);
-    else if (j <= 16) k_route<T, 16><<<grid, ROUTE_WARPS * 32, 0, s>>>(sp, logits, ld, n_tok, ids, w);
-    else k_route<T, 32><<<grid, ROUTE_WARPS * 32, 0, s>>>(sp, logits, ld, n_tok, ids, w);
-    return cudaGetLastError();
+    if (j <= 2) return launch_pdl(k_route<T, 2>, grid, ROUTE_WARPS * 32, 0, s, 0, sp, logits, ld, n_tok, ids, w);
+    if (j <= 4) return launch_pdl(k_route<T, 4>, grid, ROUTE_WARPS * 32, 0, s, 0, sp, logits, ld, n_tok, ids, w);
+    if (j <= 8) return launch_pdl(k_route<T, 8>, grid, ROUTE_WARPS * 32, 0, s, 0, sp, logits, ld, n_tok, ids, w);
+    if (j <= 16) return launch_pdl(k_route<T, 16>, grid, ROUTE_WARPS * 32, 0, s, 0, sp, logits, ld, n_tok, ids, w);
+    return launch_pdl(k_route<T, 32>, grid, ROUTE_WARPS * 32, 0, s, 0, sp, logits, ld, n_tok, ids, w);
 }
 
 cudaError_t launch_route(const RouteSpec &sp, const void *logits, int dtype, int64_t ld, int n_tok, int32_t *ids,

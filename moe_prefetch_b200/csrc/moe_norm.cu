@@ -8,7 +8,10 @@
 //
 // One pass: y and r are read once, r' and x written once, and the row stays in
 // registers over both norms (x is the norm of r' before its rounding to the
-// residual's type).  All sums and products are fp32.
+// residual's type).  All sums and products are fp32.  Bound by memory: 8,192 rows
+// of 2,048 (bf16 beside an fp32 residual, a full gate) move 235 MB in 39.5 us, 5.9
+// TB/s of a measured copy's 6.5; few rows are bound by latency (4 us for one row
+// with the combine of eight).
 #include "moe_kernels.h"
 
 #include <cuda_bf16.h>
@@ -155,16 +158,15 @@ __host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
 // memory, each thread copying and reading its own chunks (so the ring needs no
 // barrier): the kernel is bound by memory, and S - 1 rows are on their way while
 // one is in its two sums.
-// CTAs of 256 threads per SM: four, or three where the registers of a thread do
-// not fit (8,192 rows of 2,048 in bf16: 30.8 us with three and four rows in the
-// ring, 32.9 with four and three; fp32: 50.9 and 48.0; bf16 rows of 1,537: 84 and
-// 142).
-template <typename TR, int VEC, int SRC, int THREADS> constexpr int norm_ctas() {
-    return THREADS > 256 ? 1 : SRC == 0 && (VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
+// CTAs of 256 threads per SM: four, or three with more registers where that is
+// faster (8,192 rows of 2,048, bf16 beside an fp32 residual with a full gate: 40.0
+// us with three, 42.9 with four; all bf16: 26.0 and 32.9).
+template <typename TR, int VEC, int SRC, int THREADS, bool EXACT> constexpr int norm_ctas() {
+    return THREADS > 256 ? 1 : SRC == 0 && (EXACT || VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
 }
 
-template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
-__global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k_block_norm(NormArgs a) {
+template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S, bool EXACT>
+__global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXACT>()) k_block_norm(NormArgs a) {
     static_assert(S == 0 || (SRC == 0 && VEC > 1), "the ring holds aligned rows");
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ __align__(16) float part[2][32];
@@ -174,17 +176,20 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
     bool in_[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) in_[c] = at(c) < H;
-    // whether the thread has chunk c: kept, or compared anew where registers are short (8,192 rows of
-    // 2,048 in fp32: 48.1 us against 50.9; of 4,096, with 512 threads: 45.7 against 44.6)
+    // whether the thread has chunk c: all of them (EXACT: 40.0 us of the case above, 45.7 without),
+    // compared anew where registers are short, else kept
     auto in = [&](int c) {
-        if constexpr (THREADS == 256 && VEC > 1) return at(c) < H;
+        if constexpr (EXACT) return true;   // every thread has all its chunks
+        else if constexpr (THREADS == 256 && VEC > 1) return at(c) < H;
         else return in_[c];
     };
     if (threadIdx.x < 64) (&part[0][0])[threadIdx.x] = 0.0f;
     if (threadIdx.x + 32 < 64 && blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
     __syncthreads();
     pdl_enter();
-    float post[V][VEC], pre[V][VEC];        // weight + offset
+    // the factors of y and of r', but for a full gate and the row's own: (post + offset) * act(channel gate),
+    // and pre + offset
+    float post[V][VEC], pre[V][VEC];
     auto load_weights = [&]() {
 #pragma unroll
         for (int c = 0; c < V; ++c) {
@@ -194,12 +199,17 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
             if (in(c) && a.pre) norm_load(a.pre + at(c), pre[c]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                post[c][i] += a.offset;
+                post[c][i] = a.post ? post[c][i] + a.offset : 1.0f;
                 pre[c][i] = a.pre ? pre[c][i] + a.offset : 1.0f;
+            }
+            if (a.gate_kind == NORM_GATE_CHANNEL && in(c)) {
+                float g[VEC];
+                norm_load((const float *)a.gate + at(c), g);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) post[c][i] *= a.sigmoid ? norm_sigmoid(g[i]) : g[i];
             }
         }
     };
-    if (SRC == 0) load_weights();
     NormRaw<TR, VEC> r_raw[V];
     NormRaw<TY, VEC> y_raw[V], g_raw[V];
 #pragma unroll
@@ -264,6 +274,7 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
+    if (SRC == 0) load_weights();   // (behind the first rows' copies)
     int stage = 0;
     for (int64_t t = blockIdx.x; t < a.n_tok; t += gridDim.x) {
         if (S) {
@@ -325,42 +336,32 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
                     }
             }
         }
-        // the gate's factor
-        if (a.gate_kind == NORM_GATE_TOKEN) {
-            const float v = a.sigmoid ? norm_sigmoid(g_now) : g_now;
-#pragma unroll
-            for (int c = 0; c < V; ++c)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) f[c][i] = v;
-        } else if (a.gate_kind != NORM_GATE_NONE) {
-#pragma unroll
-            for (int c = 0; c < V; ++c) {
-                if (a.gate_kind == NORM_GATE_CHANNEL && in(c)) norm_load((const float *)a.gate + at(c), f[c]);
-                if (a.sigmoid) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
-                }
-            }
-        }
-        float by = a.scale;   // times scale, times post's 1 / sqrt
+        // by: what multiplies the whole row, scale * act(token gate) / sqrt(mean(y^2) + eps)
+        float by = a.scale * (a.sigmoid && a.gate_kind == NORM_GATE_TOKEN ? norm_sigmoid(g_now) : g_now);
         if (a.post) {
             float ss = 0.0f;
 #pragma unroll
             for (int c = 0; c < V; ++c)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) ss = fmaf(y[c][i] * inv_h, y[c][i], ss);
-            by = a.scale * rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
-            if (a.gate_kind == NORM_GATE_NONE) {
+            by *= rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
+        }
+        if (a.gate_kind == NORM_GATE_FULL) {
+            if (a.sigmoid) {
 #pragma unroll
                 for (int c = 0; c < V; ++c)
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) f[c][i] = post[c][i];
-            } else {
-#pragma unroll
-                for (int c = 0; c < V; ++c)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) f[c][i] *= post[c][i];
+                    for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
             }
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] *= post[c][i];
+        } else {
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] = post[c][i];
         }
         float ss = 0.0f;
         TR *ro = (TR *)a.r_out + t * a.ld_ro;
@@ -369,8 +370,7 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
             if (!in(c)) continue;       // (r is 0 there and adds nothing)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                r[c][i] = a.post || a.gate_kind != NORM_GATE_NONE ? fmaf(y[c][i] * by, f[c][i], r[c][i])
-                                                                  : fmaf(by, y[c][i], r[c][i]);
+                r[c][i] = fmaf(y[c][i] * by, f[c][i], r[c][i]);
                 ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
             }
             if (a.r_out) norm_store(ro + at(c), r[c]);
@@ -392,12 +392,13 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS>()) k
     }
 }
 
-// Rows wider than 8192, or wider than 2048 and of an odd width or alignment (VEC
-// 1): a CTA per row keeps it in shared memory as fp32 (y, then r'), and each of
-// the three passes has U chunks per thread in flight.  With a row in the registers
-// of one CTA too few threads fit an SM: 2,046 rows of 8,200 in fp32 take 64 us
-// (114 in registers), 3,928 of 4,271 in bf16 114 us (210); 10,915 of 1,537 would
-// take 106 (84).
+// Rows wider than 8192, rows of an odd width or alignment (VEC 1) wider than 2048,
+// and the combine of those of any width: a CTA per row keeps it in shared memory
+// as fp32 (y, then r'), and each of the three passes has U chunks per thread in
+// flight.  With a row in the registers of one CTA too few threads fit an SM: 2,046
+// rows of 8,200 in fp32 take 64 us (114 in registers), 3,928 of 4,271 in bf16 115
+// (210), the combine of 8 rows of 1,537 for 1,212 tokens 36 (41); 10,915 plain rows
+// of 1,537 in fp32 would take 110 (97).
 template <typename TR, typename TY, int VEC, int SRC>
 __global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
     extern __shared__ __align__(16) float row[];   // [n_embd]
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
     }
 }
 
-template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S>
+template <typename TR, typename TY, int VEC, int V, int SRC, int THREADS, int S, bool EXACT = false>
 static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     // as many CTAs as the GPU holds, at most one per row; the combine takes a CTA
     // per row, since its own loads are many enough
@@ -537,24 +538,24 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
     cudaError_t e;
     if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    int per_sm = (THREADS > 256 ? 1024 : 256 * norm_ctas<TR, VEC, SRC, THREADS>()) / threads;
+    int per_sm = (THREADS > 256 ? 1024 : 256 * norm_ctas<TR, VEC, SRC, THREADS, EXACT>()) / threads;
     const size_t smem = (size_t)S * norm_row_bytes<TR, TY>(a);
     if (S) {
         per_sm = std::min(per_sm, (int)(220 * 1024 / (smem + 2048)));
         static SmemAttr attr;
         if (smem > 40 * 1024 &&
-            (e = attr.need((const void *)k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>, (int)smem)) != cudaSuccess)
+            (e = attr.need((const void *)k_block_norm<TR, TY, VEC, V, SRC, THREADS, S, EXACT>, (int)smem)) != cudaSuccess)
             return e;
     }
     per_sm = std::min(16, std::max(1, per_sm));
-    return launch_pdl(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S>, SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads,
+    return launch_pdl(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S, EXACT>, SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads,
                       smem, s, 0, a);
 }
 
 template <typename TR, typename TY, int VEC, int SRC>
 static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const int chunks = (a.n_embd + VEC - 1) / VEC;
-    if (a.n_embd > (VEC == 1 ? 2048 : 8192)) {
+    if (a.n_embd > (VEC == 1 ? SRC == 1 ? 0 : 2048 : 8192)) {
         const size_t smem = sizeof(float) * (size_t)a.n_embd;
         static SmemAttr attr;
         cudaError_t e;
@@ -568,7 +569,11 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const int threads = ((chunks + V - 1) / V + 31) / 32 * 32;
     if constexpr (VEC > 1)
         if (threads > 256) return norm_launch<TR, TY, VEC, V, SRC, 1024, RING ? 2 : 0>(a, threads, s);
-    return norm_launch<TR, TY, VEC, V, SRC, 256, !RING ? 0 : sizeof(TR) == 2 ? 4 : 3>(a, threads, s);
+    constexpr int S = !RING ? 0 : sizeof(TR) == 2 ? 4 : 3;
+    if constexpr (VEC == 1 && SRC == 1) return cudaErrorInvalidValue;   // (k_block_norm_wide's)
+    if constexpr (RING && VEC > 2)
+        if (chunks == threads * V) return norm_launch<TR, TY, VEC, V, SRC, 256, S, true>(a, threads, s);
+    return norm_launch<TR, TY, VEC, V, SRC, 256, S>(a, threads, s);
 }
 
 template <typename TR, typename TY>

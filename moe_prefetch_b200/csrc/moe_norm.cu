@@ -9,7 +9,7 @@
 // One pass: y and r are read once, r' and x written once, and the row stays in
 // registers over both norms (x is the norm of r' before its rounding to the
 // residual's type).  All sums and products are fp32.  Bound by memory: 8,192 rows
-// of 2,048 (bf16 beside an fp32 residual, a full gate) move 235 MB in 39.5 us, 5.9
+// of 2,048 (bf16 beside an fp32 residual, a full gate) move 235 MB in 38.7 us, 6.1
 // TB/s of a measured copy's 6.5; few rows are bound by latency (4 us for one row
 // with the combine of eight).
 #include "moe_kernels.h"
@@ -160,7 +160,8 @@ __host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
 // one is in its two sums.
 // CTAs of 256 threads per SM: four, or three with more registers where that is
 // faster (8,192 rows of 2,048, bf16 beside an fp32 residual with a full gate: 40.0
-// us with three, 42.9 with four; all bf16: 26.0 and 32.9).
+// us with three, 42.9 with four; all bf16: 26.0 and 32.9; bf16 rows of 1,537: 84 and
+// 142).
 template <typename TR, int VEC, int SRC, int THREADS, bool EXACT> constexpr int norm_ctas() {
     return THREADS > 256 ? 1 : SRC == 0 && (EXACT || VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
 }
@@ -187,8 +188,11 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
     if (threadIdx.x + 32 < 64 && blockDim.x == 32) (&part[0][0])[threadIdx.x + 32] = 0.0f;
     __syncthreads();
     pdl_enter();
+    // the channel gate is folded into post in the kernels with a ring alone: without one that costs (777 rows
+    // of 1,537 with a channel gate 8.9 -> 10.6 us)
+    constexpr bool FOLD = S > 0;
     // the factors of y and of r', but for a full gate and the row's own: (post + offset) * act(channel gate),
-    // and pre + offset
+    // and pre + offset; without FOLD the channel gate stays out of post
     float post[V][VEC], pre[V][VEC];
     auto load_weights = [&]() {
 #pragma unroll
@@ -199,10 +203,10 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
             if (in(c) && a.pre) norm_load(a.pre + at(c), pre[c]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                post[c][i] = a.post ? post[c][i] + a.offset : 1.0f;
+                post[c][i] = FOLD && !a.post ? 1.0f : post[c][i] + a.offset;
                 pre[c][i] = a.pre ? pre[c][i] + a.offset : 1.0f;
             }
-            if (a.gate_kind == NORM_GATE_CHANNEL && in(c)) {
+            if (FOLD && a.gate_kind == NORM_GATE_CHANNEL && in(c)) {
                 float g[VEC];
                 norm_load((const float *)a.gate + at(c), g);
 #pragma unroll
@@ -336,32 +340,44 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
                     }
             }
         }
-        // by: what multiplies the whole row, scale * act(token gate) / sqrt(mean(y^2) + eps)
-        float by = a.scale * (a.sigmoid && a.gate_kind == NORM_GATE_TOKEN ? norm_sigmoid(g_now) : g_now);
+        // the gate's factor (a token gate's not within by: the combine equals the norm of the combined rows bit
+        // for bit, so every kernel multiplies in this order)
+        if (a.gate_kind == NORM_GATE_TOKEN) {
+            const float v = a.sigmoid ? norm_sigmoid(g_now) : g_now;
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] = v;
+        } else if (a.gate_kind == NORM_GATE_FULL || (!FOLD && a.gate_kind == NORM_GATE_CHANNEL)) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                if (!FOLD && a.gate_kind == NORM_GATE_CHANNEL && in(c)) norm_load((const float *)a.gate + at(c), f[c]);
+                if (a.sigmoid) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
+                }
+            }
+        }
+        float by = a.scale;   // times scale, times post's 1 / sqrt
         if (a.post) {
             float ss = 0.0f;
 #pragma unroll
             for (int c = 0; c < V; ++c)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) ss = fmaf(y[c][i] * inv_h, y[c][i], ss);
-            by *= rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
+            by = a.scale * rsqrtf(norm_cta_sum(ss, part[0]) + a.eps);
         }
-        if (a.gate_kind == NORM_GATE_FULL) {
-            if (a.sigmoid) {
-#pragma unroll
-                for (int c = 0; c < V; ++c)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) f[c][i] = norm_sigmoid(f[c][i]);
-            }
-#pragma unroll
-            for (int c = 0; c < V; ++c)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) f[c][i] *= post[c][i];
-        } else {
+        if (!FOLD && !a.post) {
+        } else if (a.gate_kind == NORM_GATE_NONE || (FOLD && a.gate_kind == NORM_GATE_CHANNEL)) {
 #pragma unroll
             for (int c = 0; c < V; ++c)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) f[c][i] = post[c][i];
+        } else {
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] *= post[c][i];
         }
         float ss = 0.0f;
         TR *ro = (TR *)a.r_out + t * a.ld_ro;
@@ -370,7 +386,10 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
             if (!in(c)) continue;       // (r is 0 there and adds nothing)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                r[c][i] = fmaf(y[c][i] * by, f[c][i], r[c][i]);
+                // (without post and gate f is 1 where it is set at all: the same sum, of the same rounded product)
+                r[c][i] = FOLD || a.post || a.gate_kind != NORM_GATE_NONE
+                              ? fmaf(y[c][i] * by, f[c][i], r[c][i])
+                              : __fadd_rn(__fmul_rn(by, y[c][i]), r[c][i]);
                 ss = fmaf(r[c][i] * inv_h, r[c][i], ss);
             }
             if (a.r_out) norm_store(ro + at(c), r[c]);
@@ -392,13 +411,12 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
     }
 }
 
-// Rows wider than 8192, rows of an odd width or alignment (VEC 1) wider than 2048,
-// and the combine of those of any width: a CTA per row keeps it in shared memory
-// as fp32 (y, then r'), and each of the three passes has U chunks per thread in
-// flight.  With a row in the registers of one CTA too few threads fit an SM: 2,046
-// rows of 8,200 in fp32 take 64 us (114 in registers), 3,928 of 4,271 in bf16 115
-// (210), the combine of 8 rows of 1,537 for 1,212 tokens 36 (41); 10,915 plain rows
-// of 1,537 in fp32 would take 110 (97).
+// Rows wider than 8192, or wider than 2048 and of an odd width or alignment (VEC
+// 1): a CTA per row keeps it in shared memory as fp32 (y, then r'), and each of
+// the three passes has U chunks per thread in flight.  With a row in the registers
+// of one CTA too few threads fit an SM: 2,046 rows of 8,200 in fp32 take 64 us
+// (114 in registers), 3,928 of 4,271 in bf16 114 (206); 10,915 of 1,537 would take
+// 110 (85).
 template <typename TR, typename TY, int VEC, int SRC>
 __global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
     extern __shared__ __align__(16) float row[];   // [n_embd]
@@ -555,7 +573,7 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
 template <typename TR, typename TY, int VEC, int SRC>
 static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     const int chunks = (a.n_embd + VEC - 1) / VEC;
-    if (a.n_embd > (VEC == 1 ? SRC == 1 ? 0 : 2048 : 8192)) {
+    if (a.n_embd > (VEC == 1 ? 2048 : 8192)) {
         const size_t smem = sizeof(float) * (size_t)a.n_embd;
         static SmemAttr attr;
         cudaError_t e;
@@ -570,7 +588,6 @@ static cudaError_t norm_go(const NormArgs &a, cudaStream_t s) {
     if constexpr (VEC > 1)
         if (threads > 256) return norm_launch<TR, TY, VEC, V, SRC, 1024, RING ? 2 : 0>(a, threads, s);
     constexpr int S = !RING ? 0 : sizeof(TR) == 2 ? 4 : 3;
-    if constexpr (VEC == 1 && SRC == 1) return cudaErrorInvalidValue;   // (k_block_norm_wide's)
     if constexpr (RING && VEC > 2)
         if (chunks == threads * V) return norm_launch<TR, TY, VEC, V, SRC, 256, S, true>(a, threads, s);
     return norm_launch<TR, TY, VEC, V, SRC, 256, S>(a, threads, s);

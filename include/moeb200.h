@@ -535,7 +535,8 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
  *   w: s[ids], divided by their sum when renorm (0 where that sum is 0), times
  *     scale.  The bias decides who is chosen, never the weight.
  * Ties go to the lower index.  A NaN counts as -inf when experts are compared
- * and stays NaN in the weights; a softmax over nothing but -inf is 0.  The
+ * and stays NaN in the weights (a softmax with a NaN or +inf logit is NaN for
+ * every expert); a softmax over nothing but -inf is 0.  The
  * comparison is exact: it goes by the logits where c falls with them, else by
  * c in 64 bits, so that no rounding to 32 bits decides between experts.
  * Limits: n_expert <= 512, k <= 32, n_group <= 32, a divisor of n_expert;

@@ -410,7 +410,7 @@ __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s,
         for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(MOE_FULL, sum, off);
         v = sum == 0.0 ? 0.0f : (float)(x / sum);
     } else if (s.renorm || !s.sigmoid) {
-        v = total == 0.0f ? 0.0f : v / total;
+        v = total == 0.0f && !bad ? 0.0f : v / total;   // (bad, softmax: v is NaN, and total may be 0 beside it)
     }
     w_r = v * s.scale;
 }

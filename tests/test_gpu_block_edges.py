@@ -1,0 +1,49 @@
+"""Calls of the operators around an expert layer that the first tests of them
+did not make: rows of nothing but NaN, empty pairs with weights that are no
+numbers, biases with strides, scratch between captured calls, outputs that lie
+beside their inputs, and a routing rule under the streaming lookahead.
+
+Tolerances.  u = 2^-24.  Routing weights: expf of 2 ulp (4 u) on an argument
+whose rounding is taken back, a sum of at most 32 of them in five levels (5 u
+relative, all terms positive) with 4 u of its own terms, one division (correctly
+rounded, u), the scale (u): below 20 u, and 32 u is taken, as for every routing
+test.  Everything else is compared bit for bit."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_gpu_block import BF16, F16, F32, H, U, check_route, close, randn, route_ref, router_logits  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+# ---- routing -------------------------------------------------------------------
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (4, 2, 1), (4, 2, 2)])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_rows_without_a_number(score, bias, groups, renorm):
+    """Rows of NaN, of NaN and -inf, of NaN and +inf: the weights are NaN where
+    the formula's are, renormalised or not."""
+    E, inf = 48, math.inf
+    x = 2 * randn(6, E, seed=3)
+    x[0] = math.nan
+    x[1] = math.nan
+    x[1, ::2] = -inf
+    x[2] = -inf
+    x[2, E - 1] = math.nan
+    x[3] = math.nan
+    x[3, 5] = inf
+    x[4] = -inf
+    b = 0.1 * randn(E, seed=4) if bias else None
+    check_route(x, 6, score=score, bias=b, n_group=groups[0], topk_group=groups[1], group_top=groups[2], renorm=renorm)

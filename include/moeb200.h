@@ -599,10 +599,10 @@ int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r,
                    int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok, void *stream);
 
 /* The same with y[t] = sum over j in order of w[t][j] * y_rows[pos[t][j]], then
- * + add[t] when given: moe_ep_combine's sum, bit for bit, never written to
- * memory.  All fp32; pos / w [n_tok][k], add [n_tok][n_embd].  A pos outside
- * [0, n_rows) adds nothing (-1: an empty pair).  r_out may be r; no output
- * overlaps y_rows. */
+ * + add[t] when given: moe_ep_combine's sum, bit for bit where the weights of
+ * empty pairs are finite, never written to memory.  All fp32; pos / w [n_tok][k],
+ * add [n_tok][n_embd].  A pos outside [0, n_rows) adds nothing, whatever its
+ * weight (-1: an empty pair).  r_out may be r; no output overlaps y_rows. */
 int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const float *y_rows, int64_t ld_rows,
                      int n_rows, const int32_t *pos, const float *w, int k, const float *add, float *r_out,
                      int64_t ld_ro, float *x, int64_t ld_x, int n_tok, void *stream);

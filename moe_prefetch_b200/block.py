@@ -251,7 +251,7 @@ class BlockNorm:
     def combine(self, r, y_rows, pos, w, add=None, gate=None, out=None, stream=None):
         """The same with y the combine of an expert layer's rows, y[t] = sum_j
         w[t, j] * y_rows[pos[t, j]] (+ add[t]); fp32, pos int32.  A pos
-        outside y_rows adds nothing."""
+        outside y_rows adds nothing, whatever its weight."""
         if stream is not None:
             return _on_stream(lambda: self.combine(r, y_rows, pos, w, add, gate, out), stream,
                               (r, y_rows, pos, w, add, gate, self.post, self.pre) + (out or ()))

@@ -311,12 +311,13 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int q = j0 + u < a.k ? pos[j0 + u] : -1;
-                    wj[u] = j0 + u < a.k ? w[j0 + u] : 0.0f;
+                    const bool have = q >= 0 && q < a.n_rows;
+                    wj[u] = have ? w[j0 + u] : 0.0f;   // (an empty pair's weight may be anything)
 #pragma unroll
                     for (int c = 0; c < V; ++c) {
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) v[u][c][i] = 0.0f;
-                        if (in(c) && q >= 0 && q < a.n_rows) norm_load(rows + (int64_t)q * a.ld_y + at(c), v[u][c]);
+                        if (in(c) && have) norm_load(rows + (int64_t)q * a.ld_y + at(c), v[u][c]);
                     }
                 }
 #pragma unroll
@@ -444,13 +445,14 @@ __global__ void __launch_bounds__(256) k_block_norm_wide(NormArgs a) {
             if (SRC == 1) {   // the chain of k_combine: fma from 0 in rank order, then + add
                 for (int j = 0; j < a.k; ++j) {
                     const int q = a.pos[t * a.k + j];
-                    const float w = a.w[t * a.k + j];
+                    const bool have = q >= 0 && q < a.n_rows;
+                    const float w = have ? a.w[t * a.k + j] : 0.0f;   // (an empty pair's weight may be anything)
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         float v[VEC];
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
-                        if (b + u * step < H && q >= 0 && q < a.n_rows)
+                        if (b + u * step < H && have)
                             norm_load((const float *)a.y + (int64_t)q * a.ld_y + b + u * step, v);
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) y[u][i] = __fmaf_rn(w, v[i], y[u][i]);

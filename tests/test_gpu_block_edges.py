@@ -47,3 +47,25 @@ def test_route_rows_without_a_number(score, bias, groups, renorm):
     x[4] = -inf
     b = 0.1 * randn(E, seed=4) if bias else None
     check_route(x, 6, score=score, bias=b, n_group=groups[0], topk_group=groups[1], group_top=groups[2], renorm=renorm)
+
+
+# ---- norms -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("h", [64, 2048, 1537, 1026, 8200, 16384])   # registers, odd, pairs, shared memory
+@pytest.mark.parametrize("weight", [math.nan, math.inf, -math.inf])
+def test_combine_empty_pairs_add_nothing(h, weight):
+    """A pos outside y_rows adds nothing, whatever its weight: the bits of the
+    same call with weight 0 there."""
+    from moe_prefetch_b200 import BlockNorm
+    n, k = 5, 3
+    rows, r = randn(n * k, h, seed=1), randn(n, h, seed=2)
+    pos = torch.arange(n * k, dtype=torch.int32).view(n, k)
+    pos[0, 0], pos[1, 2], pos[2, 1] = -1, n * k, -7
+    pos[3] = -1
+    empty = ((pos < 0) | (pos >= n * k)).cuda()
+    w = torch.rand(n, k, generator=torch.Generator().manual_seed(3)).cuda()
+    nm = BlockNorm(h, post=1 + 0.2 * randn(h, seed=4), pre=True)
+    want = nm.combine(r, rows, pos.cuda(), w.masked_fill(empty, 0.0))
+    got = nm.combine(r, rows, pos.cuda(), w.masked_fill(empty, weight))
+    assert torch.isfinite(want[0]).all() and torch.isfinite(want[1]).all()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

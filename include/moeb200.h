@@ -562,8 +562,10 @@ int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype, int64_t l
  * bias host or device memory, copied) for moe_layer_forward, _path, _noalloc,
  * moe_ep_route_pack and moe_block_forward; cfg NULL: softmax, top-k and
  * renormalisation again.  With the cache prior, delta is added to c of resident
- * experts after the groups are chosen.  moe_decode has the default rule built
- * in and returns MOE_ERR_UNSUPPORTED while a layer has another.  Synchronous. */
+ * experts after the groups are chosen.  The streaming lookahead ranks a layer's
+ * experts by its rule (without prior or router adapters).  moe_decode has the
+ * default rule built in and returns MOE_ERR_UNSUPPORTED while a layer has
+ * another.  Synchronous. */
 int moe_set_routing(moe_ctx *ctx, int layer, const moe_route_cfg *cfg, const float *bias);
 
 #define MOE_GATE_NONE    0

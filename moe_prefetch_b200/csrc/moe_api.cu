@@ -749,7 +749,8 @@ static volatile int32_t *host_njobs(moe_ctx *c);
 // ---- just-in-time streaming (patches/0010:951-1010 and its mover) -----------
 // After each single-token layer L of the per-layer entry points, the
 // lookahead applies the routers of L + 1 and L + 2 to L's input and claims
-// pool slots for their best non-resident experts (k_ahead_claim: jobs of
+// pool slots for their best non-resident experts, by their layer's routing
+// rule where it has one (k_ahead_claim: jobs of
 // spec 2 in the device job lists and the mapped host list).  The host mover
 // offers them to the planner with deadlines (now + (target - L) * tau -
 // margin, tau the running time per layer) and sends them earliest deadline
@@ -866,7 +867,13 @@ static int stream_after(moe_ctx *c, int layer, const float *x, cudaStream_t s) {
     if (n_targets <= 0) return stream_drain(c, s);
     for (int l = layer + 1; l <= layer + n_targets; ++l)
         if (!c->L[l].hgate_user) return stream_drain(c, s);   // nothing to stream from
-    CK(launch_ahead(c->st, c->router, x, layer + 1, n_targets, g.n_embd, g.stream_topk, g.stream_per_layer,
+    AheadRules rules{};
+    for (int t = 0; t < n_targets; ++t)
+        if (c->L[layer + 1 + t].ruled) {
+            rules.ruled[t] = 1;
+            rules.spec[t] = c->L[layer + 1 + t].rule;
+        }
+    CK(launch_ahead(c->st, c->router, x, layer + 1, n_targets, g.n_embd, g.stream_topk, g.stream_per_layer, rules,
                     c->d_scores, c->d_ahead, c->d_ahead + 32, s));
     int32_t ahead[34];
     CK(cudaMemcpyAsync(ahead, c->d_ahead, sizeof(ahead), cudaMemcpyDeviceToHost, s));

@@ -930,15 +930,17 @@ __global__ void __launch_bounds__(AHEAD_WARPS * 32) k_ahead_scores(const float *
 }
 
 // One CTA of 32 * n_targets threads: warp t takes the topk best scores of
-// target t (score descending, ties to the lower id) and keeps those its
-// layer's table says are not resident, in that order (out[t][...], count
-// n_out[t]: k_moe_ahead_post, patches/0010:407-474).  Then one thread claims
+// target t (score descending, ties to the lower id; where the target has a
+// routing rule, the topk best by its choice values among the groups it keeps)
+// and keeps those its layer's table says are not resident, in that order (out[t][...],
+// count n_out[t]: k_moe_ahead_post, patches/0010:407-474).  Then one thread claims
 // slots for them from the free pools (issue_uploads with spec 2 = streamed),
 // at most per_layer streamed jobs per layer and token, keeping max_inserts
 // slots for demand (stream_take, patches/0010:1477-1520); the claims are
 // listed for the host's mover.
 __global__ void k_ahead_claim(SlotState st, const float *__restrict__ scores, int layer0, int n_targets,
-                              int k, int per_layer, int32_t *__restrict__ out, int32_t *__restrict__ n_out) {
+                              int k, int per_layer, AheadRules rules, int32_t *__restrict__ out,
+                              int32_t *__restrict__ n_out) {
     __shared__ int32_t s_ids[2][16];
     __shared__ int s_n[2];
     const int t = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -949,7 +951,21 @@ __global__ void k_ahead_claim(SlotState st, const float *__restrict__ scores, in
         const float *sc = scores + (size_t)t * E;
         uint32_t taken = 0;       // bit j: this lane's expert lane + 32 j is picked
         int n = 0;
-        for (int r = 0; r < k; ++r) {
+        const bool ruled = rules.ruled[t] != 0;
+        if (ruled) {
+            RouteSpec sp = rules.spec[t];
+            sp.k = min(k, sp.topk_group * sp.per);   // (k <= 16; no other expert can be chosen)
+            int id_r;
+            float w_r;
+            route_warp_row<8>(sc, sp, nullptr, 0, 0.0f, false, nullptr, lane, id_r, w_r);
+            for (int r = 0; r < sp.k; ++r) {
+                const int e = __shfl_sync(MOE_FULL, id_r, r);
+                if (tbl[e] != ns) continue;
+                if (lane == 0) s_ids[t][n] = e;
+                ++n;
+            }
+        }
+        for (int r = 0; r < (ruled ? 0 : k); ++r) {
             float best = 0.0f;
             int bi = -1;
             for (int j = 0, e = lane; e < E; ++j, e += 32)
@@ -1011,15 +1027,17 @@ __global__ void k_stream_cancel(SlotState st, const int32_t *__restrict__ jobs, 
 }
 
 cudaError_t launch_ahead(const SlotState &st, const float *routers, const float *x, int layer0,
-                         int n_targets, int n_embd, int k, int per_layer, float *scores, int32_t *out,
-                         int32_t *n_out, cudaStream_t s) {
+                         int n_targets, int n_embd, int k, int per_layer, const AheadRules &rules, float *scores,
+                         int32_t *out, int32_t *n_out, cudaStream_t s) {
     if (n_targets < 1 || n_targets > 2 || k < 1 || k > 16 || per_layer < 1) return cudaErrorInvalidValue;
+    for (int t = 0; t < n_targets; ++t)
+        if (rules.ruled[t] && route_per_lane(rules.spec[t]) > 8) return cudaErrorInvalidValue;
     const int E = st.n_expert;
     k_ahead_scores<<<dim3((E + AHEAD_WARPS - 1) / AHEAD_WARPS, n_targets), AHEAD_WARPS * 32, 0, s>>>(
         routers, x, layer0, E, n_embd, scores);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    k_ahead_claim<<<1, 64, 0, s>>>(st, scores, layer0, n_targets, k, per_layer, out, n_out);
+    k_ahead_claim<<<1, 64, 0, s>>>(st, scores, layer0, n_targets, k, per_layer, rules, out, n_out);
     return cudaGetLastError();
 }
 

@@ -119,12 +119,17 @@ cudaError_t launch_step(const SlotState &st, int32_t *host_jobs, int32_t *host_n
                         cudaStream_t s);
 // just-in-time streaming: the lookahead scores of layers layer0 .. layer0 +
 // n_targets - 1 (<= 2) on one token's x, the non-resident experts among
-// their k best (out [n_targets][16], n_out [n_targets]) and the streamed
-// jobs that claim pool slots for them (at most per_layer per layer and
-// token); and the cancellation of streamed jobs (l, e, slot)
+// their k best (out [n_targets][16], n_out [n_targets]; by the target's
+// routing rule where it has one) and the streamed jobs that claim pool slots
+// for them (at most per_layer per layer and token); and the cancellation of
+// streamed jobs (l, e, slot)
+struct AheadRules {
+    int ruled[2];
+    RouteSpec spec[2];   // of the targets with ruled[t]
+};
 cudaError_t launch_ahead(const SlotState &st, const float *routers, const float *x, int layer0,
-                         int n_targets, int n_embd, int k, int per_layer, float *scores, int32_t *out,
-                         int32_t *n_out, cudaStream_t s);
+                         int n_targets, int n_embd, int k, int per_layer, const AheadRules &rules, float *scores,
+                         int32_t *out, int32_t *n_out, cudaStream_t s);
 cudaError_t launch_stream_cancel(const SlotState &st, const int32_t *jobs, int n, cudaStream_t s);
 // speculative uploads of predicted ids for layer `layer` (early issue with a predictor)
 cudaError_t launch_issue_spec(const SlotState &st, int layer, const int32_t *top, int n_top,

@@ -69,3 +69,56 @@ def test_combine_empty_pairs_add_nothing(h, weight):
     got = nm.combine(r, rows, pos.cuda(), w.masked_fill(empty, weight))
     assert torch.isfinite(want[0]).all() and torch.isfinite(want[1]).all()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- a rule under the streaming lookahead ---------------------------------------------
+
+def test_stream_lookahead_goes_by_the_rule():
+    """Layer 1 routes by bias and groups.  What the lookahead of layer 0
+    streams into layer 1, and what layer 1 then routes to, are experts of its
+    rule: with the same input on both layers nothing else ever becomes
+    resident there, and streamed experts are found in time."""
+    import time
+    from moe_prefetch_b200 import MoeCacheConfig, MoeStack, Routing
+    E, K, L = 128, 8, 2
+    src = MoeStack(n_layers=L, n_expert=E, n_ff=256)
+    src.synth_resident(seed=71, keep_router=True)
+    host = [tuple(v[:E].contiguous().cpu().pin_memory() for v in src.slot_views(il)) for il in range(L)]
+    routers = [r.clone() for r in src.routers]
+    st = MoeStack(n_layers=L, n_expert=E, n_ff=256, cache=MoeCacheConfig(
+        n_slots=64, max_inserts=8, admit="off", batch_tables=True, early_issue=True, stream=True, stream_per_layer=8,
+        stream_reserve=4))
+    # the bias turns the order of the logits around: the experts with the largest ones are never chosen
+    bias = 0.3 * randn(E, seed=9)
+    kw = dict(score="sigmoid", bias=bias, n_group=8, topk_group=3, group_top=2)
+    try:
+        for il in range(L):
+            st.set_router(il, routers[il])
+            st.set_expert_weights(il, *host[il])
+        src.routers = routers
+        st.set_routing(1, Routing(E, K, **kw))
+        allowed, raw = set(), set()
+        for t in range(12):
+            x = randn(1, H, seed=200 + t)
+            lg = router_logits(src, 1, x)
+            rid, _ = route_ref(lg, K, **kw)
+            allowed |= set(rid[0].tolist())
+            raw |= set(lg[0].topk(K)[1].tolist())
+            for il in range(L):
+                _, ids, _ = st.layer_forward(il, x)
+                torch.cuda.synchronize()
+                time.sleep(0.001)
+            assert torch.equal(ids.long().cpu(), rid)
+            st.step()
+        torch.cuda.synchronize()
+        st.step()
+        resident = st.tables(1)["slot_expert"]
+        resident = set(int(e) for e in resident[resident >= 0])
+        ss = st.stream_stats()
+        assert raw - allowed                       # (the two rules differ on these inputs)
+        assert ss["words"] > 0 and resident
+        assert resident <= allowed, sorted(resident - allowed)
+        assert ss["in_time"] > 0, ss
+    finally:
+        st.close()
+        src.close()

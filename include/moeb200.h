@@ -518,7 +518,11 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
  * no workspace, n_tok = 0 does nothing, and all of them can be captured in a
  * CUDA graph.  moe_block_forward runs them as one expert layer.
  *
- * Row strides (ld_*) count elements.  Elements of a row are contiguous. */
+ * Row strides (ld_*) count elements.  Elements of a row are contiguous.
+ *
+ * Outputs may lie between the rows of other tensors, and may be an input where
+ * the call says so: then at the same address, with the same type and stride.
+ * Any other overlap of an output is MOE_ERR_ARG. */
 #define MOE_DTYPE_F32  0
 #define MOE_DTYPE_BF16 1
 #define MOE_DTYPE_F16  2
@@ -595,8 +599,8 @@ typedef struct moe_norm {
 
 /* r, r_out [n_tok][n_embd] of r_dtype; y, x and a token or full gate of dtype.
  * r_dtype is MOE_DTYPE_F32 or dtype.  y NULL: r' = r (then no post, no gate).
- * r_out NULL (r' not wanted) or x NULL (no second norm), not both.  r_out may be
- * r, and x may be y or, without r_out, r; other overlaps are not allowed. */
+ * r_out NULL (r' not wanted) or x NULL (no second norm), not both.  r_out and x
+ * may each be r, y or a full gate, but not each other. */
 int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r, const void *y, int dtype,
                    int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok, void *stream);
 
@@ -604,7 +608,8 @@ int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r,
  * + add[t] when given: moe_ep_combine's sum, bit for bit where the weights of
  * empty pairs are finite, never written to memory.  All fp32; pos / w [n_tok][k],
  * add [n_tok][n_embd].  A pos outside [0, n_rows) adds nothing, whatever its
- * weight (-1: an empty pair).  r_out may be r; no output overlaps y_rows. */
+ * weight (-1: an empty pair).  r_out and x may each be r, add or a full gate, but
+ * not each other. */
 int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r, const float *y_rows, int64_t ld_rows,
                      int n_rows, const int32_t *pos, const float *w, int k, const float *add, float *r_out,
                      int64_t ld_ro, float *x, int64_t ld_x, int n_tok, void *stream);
@@ -627,7 +632,7 @@ typedef struct moe_adapters {
 } moe_adapters;
 
 /* out[t] = y[t] + scale[i] * B_i (A_i x[t]) with i = ids[t] (device); y NULL
- * counts as 0; out may be y, never x.  A row whose id is outside [0, n_adapters) gets
+ * counts as 0; out may be y, and overlaps nothing else.  A row whose id is outside [0, n_adapters) gets
  * y[t] (-1: a request without an adapter).  Types: x fp32, y and out fp32; or x
  * of the weights' type, y and out of that type or fp32.  A x stays in fp32. */
 int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *x, int x_dtype, int64_t ld_x,
@@ -639,8 +644,8 @@ int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *
  * routing rule -> experts -> combine, + adapters' -> the norms.
  *   norm NULL: y [n_tok][n_embd] gets the layer's output, as moe_layer_forward;
  *   norm given: y is NULL, and with the residual r [n_tok][n_embd], r_out and
- *   x_out (either may be NULL, not both; r_out may be r, and x_out may be x) get
- *   moe_combine_norm's r' and x: the input of the next block.  x_out != r_out.
+ *   x_out (either may be NULL, not both; each may be r, x or a full gate, but not
+ *   each other) get moe_combine_norm's r' and x: the input of the next block.
  * adapter_ids [n_tok] (device) choose both kinds' adapters.  Everything is fp32
  * contiguous; a token or full gate too.  ids / w are optional outputs; path,
  * prior, observation and callbacks are moe_layer_forward_path's.  Without

@@ -10,6 +10,10 @@ They are for inference: no call records a gradient.  Every call takes its work t
 stream or on ``stream``; nothing waits for the host, and the calls can be
 captured in a CUDA graph.  With ``stream`` the caller orders it after the
 producers of the inputs; the outputs are allocated for that stream.
+
+An output given with ``out`` may be an input where the call says so (the same
+memory with the same type and strides), and may lie between the rows of other
+tensors; any other overlap is a MoeError.
 """
 import ctypes as C
 
@@ -212,7 +216,8 @@ class BlockNorm:
     def __call__(self, r, y=None, gate=None, out=None, stream=None):
         """r [n, n_embd] the residual, fp32 or y's type; y the block's output
         (None: r' = r, the norm of a first block); out: (r', x) to write, r'
-        may be r (or None: not wanted) and x may be y."""
+        may be None (not wanted); each may be r, y or a full gate, but not the
+        other."""
         if stream is not None:
             return _on_stream(lambda: self(r, y, gate, out), stream,
                               (r, y, gate, self.post, self.pre) + (out or ()))
@@ -251,7 +256,8 @@ class BlockNorm:
     def combine(self, r, y_rows, pos, w, add=None, gate=None, out=None, stream=None):
         """The same with y the combine of an expert layer's rows, y[t] = sum_j
         w[t, j] * y_rows[pos[t, j]] (+ add[t]); fp32, pos int32.  A pos
-        outside y_rows adds nothing, whatever its weight."""
+        outside y_rows adds nothing, whatever its weight.  out: each may be r,
+        add or a full gate, but not the other."""
         if stream is not None:
             return _on_stream(lambda: self.combine(r, y_rows, pos, w, add, gate, out), stream,
                               (r, y_rows, pos, w, add, gate, self.post, self.pre) + (out or ()))

@@ -12,6 +12,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <list>
 #include <mutex>
 #include <string>
@@ -1741,6 +1742,51 @@ static const char *route_bad(const moe_route_cfg &r, int *code) {
 }
 
 static bool dtype_ok(int d) { return d == MOE_DTYPE_F32 || d == MOE_DTYPE_BF16 || d == MOE_DTYPE_F16; }
+static int64_t dtype_size(int d) { return d == MOE_DTYPE_F32 ? 4 : 2; }
+
+// Rows of memory that a call reads or writes: `rows` of `width` bytes, `ld` bytes
+// apart (a null pointer or no rows: nothing).
+struct Rows {
+    const void *p;
+    int64_t rows, width, ld;
+};
+static Rows flat(const void *p, int64_t bytes) { return {p, bytes > 0 ? 1 : 0, bytes, bytes}; }
+
+// The same rows: a kernel that writes a row only after it has read it may have
+// both.
+static bool same_rows(const Rows &a, const Rows &b) {
+    return a.p == b.p && a.rows == b.rows && a.width == b.width && (a.ld == b.ld || a.rows <= 1);
+}
+
+// Whether any byte belongs to both.  Rows of two tensors may alternate in one
+// buffer without meeting.
+static bool rows_meet(Rows a, Rows b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+    if (a.ld == 0) a.rows = 1;
+    if (b.ld == 0) b.rows = 1;
+    const int64_t pa = (int64_t)(intptr_t)a.p, pb = (int64_t)(intptr_t)b.p;
+    if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return false;
+    if (a.rows > b.rows) return rows_meet(b, a);
+    if (a.rows > 1 && a.ld == b.ld) {   // row j of b starts m + (q + j - i) * ld behind row i of a
+        const int64_t d = pb - pa, q = d >= 0 ? d / a.ld : -((a.ld - 1 - d) / a.ld), m = d - q * a.ld;
+        auto any = [&](int64_t s) { return -(a.rows - 1) <= s && s <= b.rows - 1; };   // whether some j - i is s
+        return (m < a.width && any(-q)) || (m + b.width > a.ld && any(-q - 1));
+    }
+    for (int64_t i = 0; i < a.rows; ++i) {   // (few calls come here)
+        const int64_t at = pa + i * a.ld;    // the first row of b that ends behind it
+        const int64_t j = b.ld > 0 && at >= pb + b.width ? (at - pb - b.width) / b.ld + 1 : 0;
+        if (j < b.rows && pb + j * b.ld < at + a.width) return true;
+    }
+    return false;
+}
+// Whether `out` meets any of `in`, of which those in `inplace` may be the same rows.
+static bool out_meets(const Rows &out, std::initializer_list<Rows> inplace, std::initializer_list<Rows> in) {
+    for (const Rows &r : inplace)
+        if (!same_rows(out, r) && rows_meet(out, r)) return true;
+    for (const Rows &r : in)
+        if (rows_meet(out, r)) return true;
+    return false;
+}
 
 extern "C" int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype, int64_t ld, int n_tok,
                          const float *bias, int32_t *ids, float *w, void *stream) {
@@ -1751,6 +1797,11 @@ extern "C" int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype
     if (const char *m = route_bad(*cfg, &code)) return fail(c, code, "moe_route: %s", m);
     if (ld < cfg->n_expert) return fail(c, MOE_ERR_ARG, "moe_route: the row stride is below n_expert");
     if (!n_tok) return MOE_OK;
+    const Rows in = {logits, n_tok, cfg->n_expert * dtype_size(dtype), ld * dtype_size(dtype)};
+    const Rows oi = flat(ids, 4 * (int64_t)n_tok * cfg->k), ow = flat(w, 4 * (int64_t)n_tok * cfg->k);
+    const Rows bi = flat(bias, 4 * (int64_t)cfg->n_expert);
+    if (out_meets(oi, {}, {in, bi, ow}) || out_meets(ow, {}, {in, bi}))
+        return fail(c, MOE_ERR_ARG, "moe_route: ids or w overlaps another tensor");
     CK(launch_route(route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
                                cfg->renorm, cfg->scale, bias),
                     logits, dtype, ld, n_tok, ids, w, (cudaStream_t)stream));
@@ -1812,6 +1863,25 @@ static NormArgs norm_args(const moe_norm &n, int n_tok) {
     return a;
 }
 
+// Whether an output of the norm meets what it may not: r_out and x may each be
+// r, y rows, a full gate or add (every thread reads its part of a row before it
+// writes there), and meet nothing else.
+static bool norm_meets(const NormArgs &a, int dt_r, int dt_y) {
+    const int64_t n = a.n_tok, h = a.n_embd, sr = dtype_size(dt_r), sy = dtype_size(dt_y);
+    const Rows none{};
+    const Rows r = {a.r, n, h * sr, a.ld_r * sr}, add = {a.add, n, h * 4, h * 4};
+    const Rows y = {a.y, a.pos ? a.n_rows : n, h * sy, a.ld_y * sy};
+    const Rows gate = a.gate_kind == MOE_GATE_FULL ? Rows{a.gate, n, h * sy, a.ld_gate * sy} : none;
+    const Rows g1 = a.gate_kind == MOE_GATE_TOKEN     ? Rows{a.gate, n, sy, a.ld_gate * sy}
+                    : a.gate_kind == MOE_GATE_CHANNEL ? flat(a.gate, 4 * h)
+                                                      : none;
+    const Rows ro = {a.r_out, n, h * sr, a.ld_ro * sr}, x = {a.x, n, h * sy, a.ld_x * sy};
+    const Rows pos = flat(a.pos, 4 * n * a.k), w = flat(a.w, 4 * n * a.k), po = flat(a.post, 4 * h), pr = flat(a.pre, 4 * h);
+    for (const Rows &o : {ro, x})
+        if (out_meets(o, {r, a.pos ? none : y, gate, add}, {a.pos ? y : none, g1, pos, w, po, pr})) return true;
+    return rows_meet(ro, x);
+}
+
 extern "C" int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, int64_t ld_r, const void *y, int dtype,
                               int64_t ld_y, void *r_out, int64_t ld_ro, void *x, int64_t ld_x, int n_tok,
                               void *stream) {
@@ -1832,6 +1902,8 @@ extern "C" int moe_block_norm(const moe_norm *nm, const void *r, int r_dtype, in
     a.y = y; a.ld_y = ld_y;
     a.r_out = r_out; a.ld_ro = ld_ro;
     a.x = x; a.ld_x = ld_x;
+    if (norm_meets(a, r_dtype, dtype))
+        return fail(c, MOE_ERR_ARG, "moe_block_norm: an output overlaps another tensor, or is one with other strides");
     CK(launch_block_norm(a, r_dtype, dtype, (cudaStream_t)stream));
     return MOE_OK;
 }
@@ -1857,6 +1929,8 @@ extern "C" int moe_combine_norm(const moe_norm *nm, const float *r, int64_t ld_r
     a.pos = pos; a.w = w; a.k = k; a.add = add;
     a.r_out = r_out; a.ld_ro = ld_ro;
     a.x = x; a.ld_x = ld_x;
+    if (norm_meets(a, DT_F32, DT_F32))
+        return fail(c, MOE_ERR_ARG, "moe_combine_norm: an output overlaps another tensor, or is one with other strides");
     CK(launch_block_norm(a, DT_F32, DT_F32, (cudaStream_t)stream));
     return MOE_OK;
 }
@@ -1874,6 +1948,13 @@ static const char *adapters_bad(const moe_adapters &s, int n_tok, int *code) {
     if (s.n_in > ADAPTER_MAX_IN) return "n_in is above 16384";
     if (s.n_adapters > ADAPTER_MAX_SET) return "more than 2047 adapters";
     return nullptr;
+}
+
+// The memory of a set, which no output may meet.
+static bool adapters_meet(const moe_adapters &s, const Rows &out) {
+    const int64_t nr = (int64_t)s.n_adapters * s.rank;
+    return out_meets(out, {}, {{s.a, nr, 2 * (int64_t)s.n_in, 2 * s.lda}, flat(s.b, 2 * nr * s.n_out), flat(s.scale, 4 * (int64_t)s.n_adapters),
+                               flat(s.ranks, 4 * (int64_t)s.n_adapters)});
 }
 
 static AdapterArgs adapter_args(const moe_adapters &s, const int32_t *ids, int n_tok) {
@@ -1899,6 +1980,11 @@ extern "C" int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, c
         return fail(c, MOE_ERR_ARG, "moe_adapters_apply: a row stride is below the row");
     if (out == x) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: out is x");
     if (y == out && ld_y != ld_out) return fail(c, MOE_ERR_ARG, "moe_adapters_apply: y and out share memory with two strides");
+    const int64_t sx = dtype_size(x_dtype), so = dtype_size(out_dtype);
+    const Rows ro = {out, n_tok, set->n_out * so, ld_out * so};
+    if (out_meets(ro, {{y, n_tok, set->n_out * so, ld_y * so}},
+                  {{x, n_tok, set->n_in * sx, ld_x * sx}, flat(ids, 4 * (int64_t)n_tok)}) || adapters_meet(*set, ro))
+        return fail(c, MOE_ERR_ARG, "moe_adapters_apply: out overlaps another tensor");
     AdapterArgs p = adapter_args(*set, ids, n_tok);
     p.x = x; p.ld_x = ld_x;
     p.y = y; p.ld_y = ld_y;
@@ -1930,6 +2016,27 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
             return fail(c, MOE_ERR_ARG, "moe_block_forward: a norm takes r and gives r_out and x_out, not y");
     } else if (n_tok && (!y || b->r || b->r_out || b->x_out)) {
         return fail(c, MOE_ERR_ARG, "moe_block_forward: without a norm there is y, and no r, r_out, x_out");
+    }
+    {
+        const int64_t n = n_tok, k = g.n_used;
+        const Rows rx = {x, n, 4 * H, 4 * H}, ry = {y, n, 4 * H, 4 * H}, ri = flat(ids, 4 * n * k), rw = flat(w, 4 * n * k);
+        const Rows ra_ids = flat(ra || la ? b->adapter_ids : nullptr, 4 * n);
+        Rows ro{}, xo{}, rr{};
+        bool bad = out_meets(ry, {}, {rx, ri, rw, ra_ids});
+        if (b->norm) {
+            NormArgs a = norm_args(*b->norm, n_tok);
+            a.r = b->r; a.r_out = b->r_out; a.x = b->x_out;
+            a.ld_r = a.ld_ro = a.ld_x = H;
+            rr = {b->r, n, 4 * H, 4 * H}; ro = {b->r_out, n, 4 * H, 4 * H}; xo = {b->x_out, n, 4 * H, 4 * H};
+            bad = norm_meets(a, MOE_DTYPE_F32, MOE_DTYPE_F32) || out_meets(ro, {rx}, {ri, rw, ra_ids}) ||
+                  out_meets(xo, {rx}, {ri, rw, ra_ids});
+        }
+        for (const Rows &o : {ri, rw}) bad = bad || out_meets(o, {}, {rx, rr, ra_ids});
+        bad = bad || rows_meet(ri, rw);
+        for (const moe_adapters *s : {ra, la})
+            if (s)
+                for (const Rows &o : {ry, ro, xo, ri, rw}) bad = bad || adapters_meet(*s, o);
+        if (n_tok && bad) return fail(c, MOE_ERR_ARG, "moe_block_forward: an output overlaps another tensor");
     }
     const bool gemm_ok = g.down_type == MOE_QTYPE_Q6_K && g.n_ff % 128 == 0 && H % 128 == 0;
     if (path == MOE_PATH_AUTO)

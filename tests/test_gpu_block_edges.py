@@ -49,6 +49,72 @@ def test_route_rows_without_a_number(score, bias, groups, renorm):
     check_route(x, 6, score=score, bias=b, n_group=groups[0], topk_group=groups[1], group_top=groups[2], renorm=renorm)
 
 
+# ---- outputs beside and over inputs ---------------------------------------------------
+
+def test_outputs_between_the_rows_of_inputs():
+    """r, y, r' and x as columns of one buffer: the bits of separate tensors."""
+    from moe_prefetch_b200 import BlockNorm
+    n, h = 400, 256
+    buf = randn(n, 4 * h, seed=1)
+    r, y, ro, x = (buf[:, i * h:(i + 1) * h] for i in range(4))
+    nm = BlockNorm(h, post=1 + 0.2 * randn(h, seed=2), pre=True, scale=0.5)
+    want = nm(r.contiguous(), y.contiguous())
+    got = nm(r, y, out=(ro, x))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("h", [64, 2048, 1537, 8200])
+def test_outputs_over_every_input_of_a_row(h):
+    """r' over y and x over r, x over a full gate, r' over add: the bits of
+    separate tensors."""
+    from moe_prefetch_b200 import BlockNorm
+    n, k = 300, 2
+    r, y, gate = (randn(n, h, seed=s) for s in (1, 2, 3))
+    nm = BlockNorm(h, post=1 + 0.2 * randn(h, seed=4), pre=True, gate_act="sigmoid", scale=0.5)
+    want = nm(r, y, gate=gate)
+    for pick in (lambda r, y, g: (y, r), lambda r, y, g: (r, g), lambda r, y, g: (g, y)):
+        t = [v.clone() for v in (r, y, gate)]
+        got = nm(t[0], t[1], gate=t[2], out=pick(*t))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    pos = torch.randperm(n * k, generator=torch.Generator().manual_seed(5)).int().view(n, k).cuda()
+    rows, w, add = randn(n * k, h, seed=6), randn(n, k, seed=7), randn(n, h, seed=8)
+    want = nm.combine(r, rows, pos, w, add=add, gate=gate)
+    t = [v.clone() for v in (r, add, gate)]
+    got = nm.combine(t[0], rows, pos, w, add=t[1], gate=t[2], out=(t[1], t[2]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_block_refuses_overlaps():
+    """Through a context: y on x, r' or x' shifted against x or r, ids on w."""
+    from moe_prefetch_b200 import BlockNorm, MoeStack, _lib
+    st = MoeStack(n_layers=1, n_expert=64, n_ff=256)
+    try:
+        st.synth_resident(seed=1)
+        n = 3
+        buf = torch.zeros(8 * n * H, device="cuda")
+        part = lambda i, shift=0: C.c_void_p(buf.data_ptr() + 4 * (i * n * H + shift))
+        ids, w = torch.zeros(n, 8, dtype=torch.int32, device="cuda"), torch.zeros(n, 8, device="cuda")
+        nm = BlockNorm(H, pre=True)
+
+        def rc(x, y=None, r=None, ro=None, xo=None, i=ids.data_ptr(), ww=w.data_ptr()):
+            b = _lib.MoeBlock()
+            if y is None:
+                b.norm, b.r, b.r_out, b.x_out = C.pointer(nm.nm), r, ro, xo
+            return st.lib.moe_block_forward(st.ctx, 0, x, n, C.byref(b), y, C.c_void_p(i), C.c_void_p(ww), 0, None)
+
+        assert rc(part(0), y=part(1)) == 0
+        assert rc(part(0), r=part(1), ro=part(1), xo=part(0)) == 0
+        assert rc(part(0), r=part(1), ro=part(2), xo=part(3)) == 0
+        for bad in (dict(y=part(0)), dict(y=part(0, 64)), dict(y=part(1), i=w.data_ptr()), dict(y=part(1), i=buf.data_ptr()),
+                    dict(y=part(1), ww=buf.data_ptr() + 4 * n * H), dict(r=part(1), ro=part(1, 8), xo=part(3)),
+                    dict(r=part(1), ro=part(2), xo=part(2, 8)), dict(r=part(1), ro=part(2), xo=part(0, 4)),
+                    dict(r=part(1), ro=part(2), xo=C.c_void_p(ids.data_ptr()))):
+            assert rc(part(0), **bad) == -1, bad
+        torch.cuda.synchronize()
+    finally:
+        st.close()
+
+
 # ---- norms -----------------------------------------------------------------------
 
 @pytest.mark.parametrize("h", [64, 2048, 1537, 1026, 8200, 16384])   # registers, odd, pairs, shared memory

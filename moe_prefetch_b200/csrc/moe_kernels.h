@@ -3,31 +3,13 @@
 #pragma once
 
 #include <cuda_runtime.h>
-#include <atomic>
 #include <cstdint>
 
 #include "moe_dev.cuh"
 #include "moe_route.cuh"
+#include "moe_smem.h"
 
 namespace moe {
-
-// cudaFuncSetAttribute of a kernel's dynamic shared memory, only where a launch on
-// this device needs more than any before (the call costs a microsecond).  One
-// object per kernel; launches may come from several threads.
-struct SmemAttr {
-    std::atomic<int> set[64];   // zero-initialised as a static
-    cudaError_t need(const void *fn, int bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        if (dev < 64 && set[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != cudaSuccess || dev >= 64) return e;
-        int old = set[dev].load(std::memory_order_relaxed);
-        while (old < bytes && !set[dev].compare_exchange_weak(old, bytes, std::memory_order_release)) {}
-        return cudaSuccess;
-    }
-};
 
 // Launch a kernel that starts with pdl_enter(): its CTAs may take their places while
 // the kernel before it on the stream is still in its last wave, and wait there

@@ -125,3 +125,60 @@ def test_route_refuses_overlaps(kw, no_gpu):
     p = {k: C.c_void_p(v) for k, v in d.items()}
     cfg = MoeRouteCfg(64, 4, 0, 1, 1, 1, 1, 1.0)
     assert lib().moe_route(C.byref(cfg), p["logits"], 0, 64, 9, p["bias"], p["ids"], p["w"], None) == ARG
+
+
+SMEM_MAIN = r"""
+// Two threads make the first calls of one kernel with different sizes.  The
+// smaller one's cudaFuncSetAttribute is held until the larger one's call has
+// ended, or for a while where that waits for the smaller one.
+#include "moe_smem.h"
+
+#include <chrono>
+#include <cstdio>
+#include <thread>
+
+static std::atomic<int> limit{0}, small_inside{0}, large_done{0};
+extern "C" cudaError_t cudaGetDevice(int *d) { *d = 0; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int bytes) {
+    if (bytes == 100) {
+        small_inside = 1;
+        for (int i = 0; i < 300 && !large_done; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+    }
+    limit = bytes;
+    return cudaSuccess;
+}
+static moe::SmemAttr attr;
+int main() {
+    std::thread a([] { attr.need(nullptr, 100); });
+    std::thread b([] {
+        while (!small_inside) std::this_thread::yield();
+        attr.need(nullptr, 150);
+        large_done = 1;
+    });
+    a.join();
+    b.join();
+    attr.need(nullptr, 150);
+    attr.need(nullptr, 120);
+    std::printf("%d\n", limit.load());
+    return limit >= 150 ? 0 : 1;
+}
+"""
+
+
+def test_shared_memory_limit_never_falls(tmp_path):
+    """A kernel's limit after first launches of two sizes from two threads
+    allows the larger one (the CUDA runtime replaced by two functions)."""
+    import os
+    import shutil
+    import subprocess
+    cuda = next((d for d in (os.environ.get("CUDA_HOME"), "/usr/local/cuda")
+                 if d and os.path.exists(os.path.join(d, "include", "cuda_runtime_api.h"))), None)
+    if cuda is None or shutil.which("g++") is None:
+        pytest.skip("no g++ or CUDA headers")
+    src, exe = tmp_path / "smem.cpp", tmp_path / "smem"
+    src.write_text(SMEM_MAIN)
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "moe_prefetch_b200", "csrc")
+    subprocess.check_call(["g++", "-std=c++17", "-pthread", "-I", os.path.join(cuda, "include"), "-I", csrc, "-o", str(exe),
+                           str(src)])
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout

@@ -650,7 +650,8 @@ int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *
  * contiguous; a token or full gate too.  ids / w are optional outputs; path,
  * prior, observation and callbacks are moe_layer_forward_path's.  Without
  * adapters, ids, w and y are its bits.  The context's scratch grows with n_tok
- * as there: one stream at a time per context, and the largest n_tok once before
+ * as there: one stream at a time per context, and the largest n_tok once (by this
+ * function, with or without adapters and norm; by each path that is named) before
  * any call is captured in a CUDA graph. */
 typedef struct moe_block {
     const moe_adapters *router_adapters;   /* n_embd -> n_expert, or NULL       */

@@ -83,8 +83,8 @@ struct moe_ctx {
     unsigned long long *ep_epoch = nullptr;   // [0] the exchange epoch, [1] the push kernel's CTA count
     bool ep_connected = false;
     float *route_bias = nullptr;       // [L][E], allocated by the first moe_set_routing with a bias
-    // moe_block_forward: router logits [n_tok][E] with router adapters, the
-    // adapters' rows [n_tok][H]
+    // moe_block_forward: room for router logits [n_tok][E] with router adapters
+    // and the adapters' rows [n_tok][H]
     float *s_block = nullptr;
     size_t s_block_cap = 0;            // floats
     // tensor-core GEMM operand tiles (fp16)
@@ -2051,7 +2051,9 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
     if ((rc = ensure_scratch(c, n_tok)) != MOE_OK) return rc;
     if (path == MOE_PATH_GEMM && (rc = ensure_gemm_scratch(c, n_tok)) != MOE_OK) return rc;
     const bool add_rows = la && b->norm;   // without a norm the adapters add to y itself
-    const size_t need = (ra ? (size_t)n_tok * E : 0) + (add_rows ? (size_t)n_tok * H : 0);
+    // for every call, with adapters or not: one call of the largest n_tok makes room for all others, and
+    // nothing that a captured call uses moves
+    const size_t need = (size_t)n_tok * (E + H);
     if (need > c->s_block_cap) {
         cudaFree(c->s_block);
         c->s_block = nullptr;
@@ -2061,7 +2063,7 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
         c->s_block_cap = need;
     }
     float *logits = ra ? c->s_block : nullptr;
-    float *delta = add_rows ? c->s_block + (ra ? (size_t)n_tok * E : 0) : nullptr;
+    float *delta = add_rows ? c->s_block + (size_t)n_tok * E : nullptr;
     cudaStream_t s = (cudaStream_t)stream;
     if (g.stream && n_tok == 1 && (rc = stream_enter(c, layer, s)) != MOE_OK) return rc;
     int32_t *ids_d = ids ? ids : c->s_ids;

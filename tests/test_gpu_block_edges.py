@@ -188,3 +188,42 @@ def test_stream_lookahead_goes_by_the_rule():
     finally:
         st.close()
         src.close()
+
+
+# ---- scratch between captured calls ------------------------------------------------------
+
+def test_one_plain_call_makes_room_for_every_captured_one():
+    """The largest n_tok once, without adapters.  Then calls with router
+    adapters, with layer adapters and with both are captured and replayed
+    between eager calls of the other kinds: none allocates, and every replay has
+    the eager call's bits."""
+    from moe_prefetch_b200 import AdapterSet, BlockNorm, MoeStack
+    st = MoeStack(n_layers=1, n_expert=64, n_ff=256)
+    try:
+        st.synth_resident(seed=3)
+        n = 24
+        x, r = randn(n, H, seed=1), randn(n, H, seed=2)
+        ids = torch.randint(-1, 3, (n,), generator=torch.Generator().manual_seed(4)).int().cuda()
+        ra = AdapterSet((randn(3, 8, H, seed=5) / 45).to(BF16), randn(3, 64, 8, seed=6).to(BF16))
+        la = AdapterSet((randn(3, 8, H, seed=7) / 45).to(BF16), randn(3, H, 8, seed=8).to(BF16))
+        nm = BlockNorm(H, post=1 + 0.2 * randn(H, seed=9), pre=True)
+        st.block_forward(0, x)
+        torch.cuda.synchronize()
+        calls = [lambda kw=kw, m=m: st.block_forward(0, x[:m], r=r[:m], norm=nm, adapter_ids=ids[:m], **kw)
+                 for kw, m in ((dict(router_adapters=ra), n), (dict(adapters=la), n - 1),
+                               (dict(router_adapters=ra, adapters=la), n))]
+        graphs = []
+        for call in calls:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = call()
+            graphs.append((g, out))
+        for turn in range(2):
+            x.copy_(randn(n, H, seed=20 + turn))
+            want = [call() for call in calls]
+            for (g, out), w in zip(graphs, want):
+                g.replay()
+                assert all(torch.equal(a, b) for a, b in zip(out, w))
+        torch.cuda.synchronize()
+    finally:
+        st.close()

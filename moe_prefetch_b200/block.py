@@ -108,8 +108,9 @@ class Routing:
         check(self.lib.moe_route(C.byref(self.cfg), None, 0, n_expert, 0, None, None, None, None), None, "moe_route")
         if bias is not None and (bias.shape != (n_expert,) or bias.dtype != torch.float32):
             raise ValueError(f"bias must be fp32 [{n_expert}], got {bias.dtype} {tuple(bias.shape)}")
-        self.bias = None if bias is None else bias.contiguous()
-        self.bias_ptr = None if bias is None else self.bias.data_ptr()
+        self.bias = bias
+        # (the bias of a strided tensor is gathered by every call)
+        self.bias_ptr = None if bias is None or not bias.is_contiguous() else bias.data_ptr()
         self.cfg_ref = C.byref(self.cfg)
 
     def __call__(self, logits, out=None, stream=None):
@@ -123,9 +124,13 @@ class Routing:
                 return self(logits, out)
         ld = _rows(logits, "logits", self.n_expert)
         device, n, k = logits.device, logits.shape[0], self.k
-        bias = self.bias
-        if bias is not None and bias.device != device:
-            raise ValueError(f"the bias is on {bias.device}, the logits are on {device}")
+        bias, bias_ptr = self.bias, self.bias_ptr
+        if bias is not None:
+            if bias.device != device:
+                raise ValueError(f"the bias is on {bias.device}, the logits are on {device}")
+            if bias_ptr is None:
+                bias = bias.contiguous()
+                bias_ptr = bias.data_ptr()
         if out is None:
             ids = torch.empty(n, k, dtype=torch.int32, device=device)
             w = torch.empty(n, k, dtype=torch.float32, device=device)
@@ -135,7 +140,7 @@ class Routing:
                     or not ids.is_contiguous() or not w.is_contiguous()):
                 raise ValueError(f"out must be contiguous int32 and fp32 [{n}, {k}]")
             _same_device(device, ids=ids, w=w)
-        rc = self.lib.moe_route(self.cfg_ref, logits.data_ptr(), DTYPES[logits.dtype], ld, n, self.bias_ptr,
+        rc = self.lib.moe_route(self.cfg_ref, logits.data_ptr(), DTYPES[logits.dtype], ld, n, bias_ptr,
                                 ids.data_ptr(), w.data_ptr(), _raw_stream(index))
         if rc:
             check(rc, None, "moe_route")

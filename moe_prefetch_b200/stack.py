@@ -319,8 +319,8 @@ class MoeStack:
         if routing is None:
             self._ck(self.lib.moe_set_routing(self.ctx, layer, None, None), "moe_set_routing")
             return
-        self._ck(self.lib.moe_set_routing(self.ctx, layer, C.byref(routing.cfg), _ptr(routing.bias)),
-                 "moe_set_routing")
+        bias = None if routing.bias is None else routing.bias.contiguous()
+        self._ck(self.lib.moe_set_routing(self.ctx, layer, C.byref(routing.cfg), _ptr(bias)), "moe_set_routing")
 
     def block_forward(self, layer, x, r=None, norm=None, gate=None, adapter_ids=None, router_adapters=None,
                       adapters=None, out=None, path="auto", stream=None):

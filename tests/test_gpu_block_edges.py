@@ -227,3 +227,41 @@ def test_one_plain_call_makes_room_for_every_captured_one():
         torch.cuda.synchronize()
     finally:
         st.close()
+
+
+# ---- arguments -------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def one_layer():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from moe_prefetch_b200 import MoeStack
+    st = MoeStack(n_layers=1, n_expert=64, n_ff=256)
+    st.synth_resident(seed=6, keep_router=True)
+    yield st
+    st.close()
+
+
+def test_route_bias_with_a_stride_is_read_at_every_call():
+    from moe_prefetch_b200 import Routing
+    E = 64
+    table = 0.3 * randn(E, 3, seed=1)
+    x = randn(9, E, seed=2)
+    rt = Routing(E, 4, score="sigmoid", bias=table[:, 1])
+    for turn in range(2):
+        ids, w = rt(x)
+        rid, rw = route_ref(x, 4, score="sigmoid", bias=table[:, 1])
+        assert torch.equal(ids.long().cpu(), rid)
+        table.copy_(0.3 * randn(E, 3, seed=7))
+
+
+def test_layer_rule_takes_a_bias_with_a_stride(one_layer):
+    from moe_prefetch_b200 import Routing
+    bias = 0.3 * randn(64, 2, seed=3)[:, 1]
+    x = randn(4, H, seed=4)
+    rid, _ = route_ref(router_logits(one_layer, 0, x), 8, score="sigmoid", bias=bias)
+    one_layer.set_routing(0, Routing(64, 8, score="sigmoid", bias=bias))
+    try:
+        assert torch.equal(one_layer.layer_forward(0, x)[1].long().cpu(), rid)
+    finally:
+        one_layer.set_routing(0, None)

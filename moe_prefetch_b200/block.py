@@ -117,7 +117,7 @@ class Routing:
         """logits [n, n_expert] (fp32, bf16 or fp16) -> (ids, w); out: the
         (ids, w) to write."""
         if stream is not None:
-            return _on_stream(lambda: self(logits, out), stream, (logits, self.bias) + (out or ()))
+            return _on_stream(lambda: self(logits, out), stream, (logits, self.bias, *(out or ())))
         index = logits.get_device()
         if index >= 0 and index != _current_device():
             with torch.cuda.device(index):
@@ -225,7 +225,7 @@ class BlockNorm:
         other."""
         if stream is not None:
             return _on_stream(lambda: self(r, y, gate, out), stream,
-                              (r, y, gate, self.post, self.pre) + (out or ()))
+                              (r, y, gate, self.post, self.pre, *(out or ())))
         index = r.get_device()
         if index >= 0 and index != _current_device():
             with torch.cuda.device(index):
@@ -265,7 +265,7 @@ class BlockNorm:
         add or a full gate, but not the other."""
         if stream is not None:
             return _on_stream(lambda: self.combine(r, y_rows, pos, w, add, gate, out), stream,
-                              (r, y_rows, pos, w, add, gate, self.post, self.pre) + (out or ()))
+                              (r, y_rows, pos, w, add, gate, self.post, self.pre, *(out or ())))
         index = r.get_device()
         if index >= 0 and index != _current_device():
             with torch.cuda.device(index):

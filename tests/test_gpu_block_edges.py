@@ -265,3 +265,23 @@ def test_layer_rule_takes_a_bias_with_a_stride(one_layer):
         assert torch.equal(one_layer.layer_forward(0, x)[1].long().cpu(), rid)
     finally:
         one_layer.set_routing(0, None)
+
+
+def test_outputs_in_a_list_on_a_stream():
+    """out as a list, with a stream of the call's own."""
+    from moe_prefetch_b200 import BlockNorm, Routing
+    x, r = randn(7, 64, seed=1), randn(7, 64, seed=2)
+    rt, nm = Routing(64, 4), BlockNorm(64, pre=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    out = [torch.empty(7, 4, dtype=torch.int32, device="cuda"), torch.empty(7, 4, device="cuda")]
+    ro = [torch.empty_like(r), torch.empty_like(r)]
+    co = [torch.empty_like(r), torch.empty_like(r)]
+    pos, w = torch.arange(7, dtype=torch.int32, device="cuda").view(7, 1), torch.ones(7, 1, device="cuda")
+    torch.cuda.synchronize()
+    rt(x, out=out, stream=s)
+    nm(r, x, out=ro, stream=s)
+    nm.combine(r, x, pos, w, out=co, stream=s)
+    s.synchronize()
+    for got, want in ((out, rt(x)), (ro, nm(r, x)), (co, nm.combine(r, x, pos, w))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

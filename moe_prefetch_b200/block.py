@@ -94,8 +94,9 @@ class Routing:
 
     ``routing(logits)`` -> ids int32 [n, k], w fp32 [n, k].  Ties go to the
     lower expert; a logit of -inf has score 0, and with a bias of -inf an expert
-    is chosen last.  The bias tensor is read at every call, so that a change of
-    its values is seen (MoeStack.set_routing copies it)."""
+    is chosen last.  The bias tensor's memory is read at every call, so that a
+    change of its values in place is seen (MoeStack.set_routing copies it);
+    other memory that the tensor is given later (``bias.data = ...``) is not."""
 
     def __init__(self, n_expert, k, score="softmax", bias=None, n_group=1, topk_group=None, group_top=1,
                  renorm=True, scale=1.0):
@@ -108,7 +109,7 @@ class Routing:
         check(self.lib.moe_route(C.byref(self.cfg), None, 0, n_expert, 0, None, None, None, None), None, "moe_route")
         if bias is not None and (bias.shape != (n_expert,) or bias.dtype != torch.float32):
             raise ValueError(f"bias must be fp32 [{n_expert}], got {bias.dtype} {tuple(bias.shape)}")
-        self.bias = bias
+        self.bias = None if bias is None else bias.detach()   # (keeps the memory whose address is used)
         # (the bias of a strided tensor is gathered by every call)
         self.bias_ptr = None if bias is None or not bias.is_contiguous() else bias.data_ptr()
         self.cfg_ref = C.byref(self.cfg)
@@ -155,7 +156,8 @@ class BlockNorm:
         x  = r' / sqrt(mean(r'^2) + eps) * (pre + weight_offset)
 
     post, pre: fp32 [n_embd] weights, or None (post None: no norm after the
-    block; pre None: no x; pre True: x with weight 1).  ``norm(r, y)`` and
+    block; pre None: no x; pre True: x with weight 1); their memory is read at
+    every call, as a Routing's bias is.  ``norm(r, y)`` and
     ``norm.combine(r, y_rows, pos, w)`` return (r', x)."""
 
     def __init__(self, n_embd, post=None, pre=None, gate_act="none", scale=1.0, eps=1e-6, weight_offset=0.0):
@@ -164,7 +166,8 @@ class BlockNorm:
         self.lib = _lib.load()
         self.n_embd = n_embd
         self.with_x = pre is not None and pre is not False
-        self.post, self.pre = post, pre if isinstance(pre, torch.Tensor) else None
+        self.post = None if post is None else post.detach()
+        self.pre = pre.detach() if isinstance(pre, torch.Tensor) else None
         for name, t in (("post", self.post), ("pre", self.pre)):
             if t is not None and (t.shape != (n_embd,) or t.dtype != torch.float32 or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous fp32 [{n_embd}]")

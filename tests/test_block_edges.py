@@ -182,3 +182,15 @@ def test_shared_memory_limit_never_falls(tmp_path):
                            str(src)])
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout
+
+
+def test_weights_given_other_memory_are_not_dangling():
+    """A weight whose tensor is given other memory (as moving a module does)
+    keeps the memory that its address was taken from."""
+    from moe_prefetch_b200 import BlockNorm, Routing
+    post, pre, bias = (torch.nn.Parameter(torch.zeros(64)) for _ in range(3))
+    nm, rt = BlockNorm(64, post=post, pre=pre), Routing(64, 4, bias=bias)
+    for t in (post, pre, bias):
+        t.data = torch.ones(64)
+    assert (nm.post.data_ptr(), nm.pre.data_ptr()) == (nm.nm.post, nm.nm.pre) and nm.with_x
+    assert rt.bias.data_ptr() == rt.bias_ptr

@@ -529,6 +529,7 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
 
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
+#define MOE_SCORE_MASKED  0x100    /* with either: a logit of -inf masks its expert */
 
 /* A routing rule.  With scores s = softmax(logits) or sigmoid(logits) and
  * choice values c = s + bias (c = s without bias):
@@ -540,7 +541,11 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
  *     scale.  The bias decides who is chosen, never the weight.
  * Ties go to the lower index.  A NaN counts as -inf when experts are compared
  * and stays NaN in the weights (a softmax with a NaN or +inf logit is NaN for
- * every expert); a softmax over nothing but -inf is 0.  The
+ * every expert); a softmax over nothing but -inf is 0.  A logit of -inf is a score
+ * of 0, so that a bias can still choose its expert, with weight 0.  With
+ * MOE_SCORE_MASKED such an expert's c is -inf whatever its bias: it is chosen
+ * last, where fewer than k others are left, and a group's sum of two leaves it
+ * out.  The
  * comparison is exact: it goes by the logits where c falls with them, else by
  * c in 64 bits, so that no rounding to 32 bits decides between experts.
  * Limits: n_expert <= 512, k <= 32, n_group <= 32, a divisor of n_expert;
@@ -549,7 +554,7 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
  * moe_router_run. */
 typedef struct moe_route_cfg {
     int32_t n_expert, k;
-    int32_t score;             /* MOE_SCORE_*                                   */
+    int32_t score;             /* MOE_SCORE_SOFTMAX or _SIGMOID (| _MASKED)     */
     int32_t n_group;           /* 1: no groups                                  */
     int32_t topk_group;
     int32_t group_top;         /* 1 or 2                                        */

@@ -24,6 +24,7 @@ from ._lib import MoeAdapters, MoeNorm, MoeRouteCfg, check
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 SCORES = {"softmax": 0, "sigmoid": 1}
+SCORE_MASKED = 0x100
 ACTS = {"none": 0, "sigmoid": 1}
 _ROWS = torch.contiguous_format
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
@@ -90,7 +91,9 @@ class Routing:
     balance that decides who is chosen but never the weight, n_group groups of
     which the topk_group best are kept (by their largest value, or with
     group_top 2 by the sum of their two largest), the k best experts, weights
-    divided by their sum (renorm) and multiplied by scale.
+    divided by their sum (renorm) and multiplied by scale.  With masked a logit of
+    -inf switches its expert off for that token: it is chosen last, whatever its
+    bias (without, its score is 0 and the bias may choose it, with weight 0).
 
     ``routing(logits)`` -> ids int32 [n, k], w fp32 [n, k].  Ties go to the
     lower expert; a logit of -inf has score 0, and with a bias of -inf an expert
@@ -99,13 +102,13 @@ class Routing:
     other memory that the tensor is given later (``bias.data = ...``) is not."""
 
     def __init__(self, n_expert, k, score="softmax", bias=None, n_group=1, topk_group=None, group_top=1,
-                 renorm=True, scale=1.0):
+                 renorm=True, scale=1.0, masked=False):
         if score not in SCORES:
             raise ValueError(f"unknown score {score!r}")
         self.lib = _lib.load()
         self.n_expert, self.k = n_expert, k
-        self.cfg = MoeRouteCfg(n_expert, k, SCORES[score], n_group, n_group if topk_group is None else topk_group,
-                               group_top, int(bool(renorm)), scale)
+        self.cfg = MoeRouteCfg(n_expert, k, SCORES[score] | (SCORE_MASKED if masked else 0), n_group,
+                               n_group if topk_group is None else topk_group, group_top, int(bool(renorm)), scale)
         check(self.lib.moe_route(C.byref(self.cfg), None, 0, n_expert, 0, None, None, None, None), None, "moe_route")
         if bias is not None and (bias.shape != (n_expert,) or bias.dtype != torch.float32):
             raise ValueError(f"bias must be fp32 [{n_expert}], got {bias.dtype} {tuple(bias.shape)}")

@@ -722,7 +722,7 @@ static cudaError_t route_tokens(moe_ctx *c, int layer, const float *x, int n_tok
     const int prior = one && g.cache_prior > 0.0f, obs = one ? layer : -1;
     const int32_t *pub = cached ? c->st.slot_expert + c->slot_off[layer] : nullptr;
     if (logits) {
-        const RouteSpec sp = m.ruled ? m.rule : route_spec(g.n_expert, g.n_used, 0, 1, 1, 1, 1, 1.0f, nullptr);
+        const RouteSpec sp = m.ruled ? m.rule : route_spec(g.n_expert, g.n_used, 0, 1, 1, 1, 1, 0, 1.0f, nullptr);
         return one ? launch_route_one(sp, logits, ids, w, table, m.ns, delta, prior, c->st, layer, pub, s)
                    : launch_route(sp, logits, DT_F32, g.n_expert, n_tok, ids, w, s);
     }
@@ -1729,7 +1729,8 @@ extern "C" int moe_decode_info(const moe_ctx *c, int32_t *out, int n) {
 static const char *route_bad(const moe_route_cfg &r, int *code) {
     *code = MOE_ERR_ARG;
     if (r.n_expert <= 0 || r.k <= 0 || r.n_group <= 0 || r.topk_group <= 0) return "a non-positive size";
-    if (r.score != MOE_SCORE_SOFTMAX && r.score != MOE_SCORE_SIGMOID) return "an unknown score";
+    const int32_t score = r.score & ~MOE_SCORE_MASKED;
+    if (score != MOE_SCORE_SOFTMAX && score != MOE_SCORE_SIGMOID) return "an unknown score";
     if (r.group_top != 1 && r.group_top != 2) return "group_top must be 1 or 2";
     if (r.n_expert % r.n_group) return "n_group does not divide n_expert";
     if (r.topk_group > r.n_group) return "topk_group is above n_group";
@@ -1739,6 +1740,11 @@ static const char *route_bad(const moe_route_cfg &r, int *code) {
     if (r.k > ROUTE_MAX_K) return "k is above 32";
     if (r.n_group > ROUTE_MAX_GROUP) return "n_group is above 32";
     return nullptr;
+}
+
+static RouteSpec spec_of(const moe_route_cfg &r, const float *bias) {
+    return route_spec(r.n_expert, r.k, (r.score & ~MOE_SCORE_MASKED) == MOE_SCORE_SIGMOID, r.n_group, r.topk_group,
+                      r.group_top, r.renorm, (r.score & MOE_SCORE_MASKED) != 0, r.scale, bias);
 }
 
 static bool dtype_ok(int d) { return d == MOE_DTYPE_F32 || d == MOE_DTYPE_BF16 || d == MOE_DTYPE_F16; }
@@ -1802,9 +1808,7 @@ extern "C" int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype
     const Rows bi = flat(bias, 4 * (int64_t)cfg->n_expert);
     if (out_meets(oi, {}, {in, bi, ow}) || out_meets(ow, {}, {in, bi}))
         return fail(c, MOE_ERR_ARG, "moe_route: ids or w overlaps another tensor");
-    CK(launch_route(route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
-                               cfg->renorm, cfg->scale, bias),
-                    logits, dtype, ld, n_tok, ids, w, (cudaStream_t)stream));
+    CK(launch_route(spec_of(*cfg, bias), logits, dtype, ld, n_tok, ids, w, (cudaStream_t)stream));
     return MOE_OK;
 }
 
@@ -1834,8 +1838,7 @@ extern "C" int moe_set_routing(moe_ctx *c, int layer, const moe_route_cfg *cfg, 
         CK(cudaMemcpy(dst, bias, sizeof(float) * g.n_expert, cudaMemcpyDefault));
         CK(cudaDeviceSynchronize());
     }
-    m.rule = route_spec(cfg->n_expert, cfg->k, cfg->score, cfg->n_group, cfg->topk_group, cfg->group_top,
-                        cfg->renorm, cfg->scale, dst);
+    m.rule = spec_of(*cfg, dst);
     m.ruled = true;
     return MOE_OK;
 }

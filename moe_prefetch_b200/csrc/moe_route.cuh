@@ -18,9 +18,10 @@ namespace moe {
 //           largest) keep their experts;
 //   ids:    the k largest c of the kept experts, in order;
 //   w:      s[ids] (divided by their sum), times scale.
-// Ties go to the lower index, and a NaN counts as -inf, everywhere.
+// Ties go to the lower index, and a NaN counts as -inf, everywhere.  With `masked`
+// an expert whose logit is -inf has c = -inf, and a group's sum leaves out -inf.
 struct RouteSpec {
-    int n_expert, k, sigmoid, n_group, topk_group, group_top, renorm;
+    int n_expert, k, sigmoid, n_group, topk_group, group_top, renorm, masked;
     int per;       // experts per group
     int log_lanes; // 2^log_lanes lanes per group: the largest power of two <= 32 / n_group
     float scale;
@@ -33,8 +34,8 @@ constexpr int ROUTE_MAX_K = 32;
 
 // The rule of checked arguments, with its derived fields.
 inline RouteSpec route_spec(int n_expert, int k, int sigmoid, int n_group, int topk_group, int group_top, int renorm,
-                            float scale, const float *bias) {
-    RouteSpec s{n_expert, k, sigmoid, n_group, topk_group, group_top, renorm, n_expert / n_group, 5, scale, bias};
+                            int masked, float scale, const float *bias) {
+    RouteSpec s{n_expert, k, sigmoid, n_group, topk_group, group_top, renorm, masked, n_expert / n_group, 5, scale, bias};
     while (n_group << s.log_lanes > 32) --s.log_lanes;
     return s;
 }
@@ -95,7 +96,7 @@ __device__ __forceinline__ V route_group(const V (&c)[J], int count, const Route
         b2 = max(min(b1, o1), max(b2, o2));
         b1 = max(b1, o1);
     }
-    return route_clean(s.group_top == 2 && s.per > 1 ? b1 + b2 : b1);
+    return route_clean(s.group_top == 2 && s.per > 1 && !(s.masked && b2 == -(V)INFINITY) ? b1 + b2 : b1);
 }
 
 // True when this lane's group (its key gk, the same in all its lanes) is among
@@ -314,7 +315,10 @@ __device__ __forceinline__ int route_exact(const float (&l)[J], const RouteSpec 
     }
 #pragma unroll
     for (int j = 0; j < J; ++j)
-        if (j < me.count) c[j] = route_clean(c[j] * inv + (s.bias ? (double)s.bias[me.expert(j)] : 0.0));
+        if (j < me.count) {
+            c[j] = route_clean(c[j] * inv + (s.bias ? (double)s.bias[me.expert(j)] : 0.0));
+            if (s.masked && l[j] == -INFINITY) c[j] = -(double)INFINITY;
+        }
     const bool kept = s.n_group == 1 || route_group_kept(s, route_key(route_group(c, me.count, s)), me.group);
     uint32_t alive = 0;
 #pragma unroll
@@ -336,7 +340,8 @@ __device__ __forceinline__ float route_load(const __half *p) { return __half2flo
 // Without bias and prior the choice values fall with the logits, which are
 // compared as they are.  Otherwise 32-bit scores decide where they are far
 // enough apart (route_fast: about 998 tokens in 1000), and 64-bit scores where
-// their rounding could decide between two experts.
+// their rounding could decide between two experts, and for tokens with masked
+// experts.
 //
 // The weights are formed in 32 bits (expf 4 u with the rounding of l - mx taken
 // back, k - 1 additions in five levels, two divisions, scale: below 20 u); where
@@ -378,7 +383,14 @@ __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s,
         id_r = route_topk(key, s, me, lane);
         bad = !s.sigmoid && is_bad();
     } else {
-        id_r = prior ? -1 : route_fast<J>(l, s, me, mx, lane, total);   // (no bad logits where it succeeds)
+        bool exact = prior;
+        if (s.masked) {
+            bool off = false;
+#pragma unroll
+            for (int j = 0; j < J; ++j) off = off || (j < me.count && l[j] == -INFINITY);
+            exact = __any_sync(MOE_FULL, off) || prior;
+        }
+        id_r = exact ? -1 : route_fast<J>(l, s, me, mx, lane, total);   // (no bad logits where it succeeds)
         if (__any_sync(MOE_FULL, id_r < 0)) {
             bad = is_bad();
             id_r = route_exact<J>(l, s, me, mx, bad, table, ns, delta, prior, pub, lane);

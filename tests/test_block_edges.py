@@ -194,3 +194,11 @@ def test_weights_given_other_memory_are_not_dangling():
         t.data = torch.ones(64)
     assert (nm.post.data_ptr(), nm.pre.data_ptr()) == (nm.nm.post, nm.nm.pre) and nm.with_x
     assert rt.bias.data_ptr() == rt.bias_ptr
+
+
+def test_masked_scores_are_checked():
+    from moe_prefetch_b200 import Routing
+    from test_block_ops import route_rc
+    for score, code in ((0x100, 0), (0x101, 0), (0x102, ARG), (0x200, ARG), (-1, ARG)):
+        assert route_rc(score=score, n_tok=0) == code
+    assert Routing(64, 4, masked=True).cfg.score == 0x100 and Routing(64, 4, "sigmoid").cfg.score == 1

@@ -49,6 +49,81 @@ def test_route_rows_without_a_number(score, bias, groups, renorm):
     check_route(x, 6, score=score, bias=b, n_group=groups[0], topk_group=groups[1], group_top=groups[2], renorm=renorm)
 
 
+def masked_ref(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_top=1, renorm=True, scale=1.0):
+    """A masked rule token by token in 64 bits: an expert whose logit is -inf
+    (or NaN) compares as -inf, a group's sum has only what is left of it."""
+    L = logits.double().cpu().numpy()
+    b = np.zeros(L.shape[1]) if bias is None else bias.double().cpu().numpy()
+    ids, ws = [], []
+    with np.errstate(all="ignore"):
+        for l in L:
+            off = np.isneginf(l) | np.isnan(l)
+            e = np.exp(l - l.max()) if np.isfinite(l.max()) else np.zeros_like(l)
+            s = 1 / (1 + np.exp(-l)) if score == "sigmoid" else e / e.sum() if e.sum() else e
+            by_logit = bias is None and (n_group == 1 or group_top == 1)
+            c = np.where(off, -np.inf, l if by_logit else s + b)
+            per = len(l) // n_group
+            strength = []
+            for g in range(n_group):
+                best = sorted(c[g * per:(g + 1) * per], reverse=True)[:group_top]
+                strength.append(sum(v for v in best if v > -np.inf) if best[0] > -np.inf else -np.inf)
+            keep = sorted(range(n_group), key=lambda g: (-strength[g], g))[:topk_group]
+            pick = sorted((i for i in range(len(l)) if i // per in keep), key=lambda i: (-c[i], i))[:k]
+            w = s[pick]
+            if renorm:
+                w = w / w.sum() if w.sum() else 0 * w
+            ids.append(pick)
+            ws.append(w * np.float64(np.float32(scale)))
+    return torch.tensor(np.array(ids)), torch.tensor(np.array(ws))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [None, 0.5, -5.0])
+@pytest.mark.parametrize("E,k,groups", [(48, 6, (1, 1, 1)), (48, 6, (4, 2, 1)), (48, 6, (4, 2, 2)), (157, 6, (1, 1, 1)),
+                                        (256, 8, (4, 2, 2)), (512, 16, (1, 1, 1)), (493, 5, (17, 3, 2)), (32, 4, (32, 8, 2))])
+def test_masked_experts_are_chosen_last(score, bias, E, k, groups):
+    """Under a positive bias no expert that a token may not use is chosen while
+    others are left, in every layout of the lanes; rows with one, with none and
+    with all experts left."""
+    from moe_prefetch_b200 import Routing
+    n = 65
+    x = 2 * randn(n, E, seed=E)
+    g = torch.Generator().manual_seed(E)
+    x.scatter_(1, torch.randint(0, E, (n, max(1, E // 3)), generator=g).cuda(), -math.inf)
+    x[0] = -math.inf
+    x[1] = -math.inf
+    x[1, E // 2] = 1.0
+    x[2] = 2 * randn(E, seed=1)
+    x[3, E // 2:] = -math.inf
+    b = None if bias is None else bias + 0.2 * randn(E, seed=2)
+    kw = dict(score=score, bias=b, n_group=groups[0], topk_group=groups[1], group_top=groups[2], scale=1.5)
+    for renorm in (True, False):
+        ids, w = Routing(E, k, masked=True, renorm=renorm, **kw)(x)
+        rid, rw = masked_ref(x, k, renorm=renorm, **kw)
+        assert torch.equal(ids.long().cpu(), rid)
+        close(w, rw, 32 * U * rw.abs(), "w")
+    if groups[0] == 1:
+        left = torch.isfinite(x).sum(1, keepdim=True).clamp(max=k).cpu()
+        off = torch.isneginf(x).gather(1, ids.long()).cpu()
+        assert torch.equal(off, torch.arange(k)[None] >= left)
+
+
+def test_a_layer_takes_a_masked_rule():
+    """A rule with masks on a layer whose logits have none: the plain rule."""
+    from moe_prefetch_b200 import MoeStack, Routing
+    st = MoeStack(n_layers=1, n_expert=64, n_ff=256)
+    try:
+        st.synth_resident(seed=2)
+        x, b = randn(5, H, seed=1), 0.2 * randn(64, seed=2)
+        got = []
+        for masked in (False, True):
+            st.set_routing(0, Routing(64, 8, score="sigmoid", bias=b, n_group=4, topk_group=2, group_top=2, masked=masked))
+            got.append(st.layer_forward(0, x))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+    finally:
+        st.close()
+
+
 # ---- outputs beside and over inputs ---------------------------------------------------
 
 def test_outputs_between_the_rows_of_inputs():

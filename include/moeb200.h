@@ -639,7 +639,10 @@ typedef struct moe_adapters {
 /* out[t] = y[t] + scale[i] * B_i (A_i x[t]) with i = ids[t] (device); y NULL
  * counts as 0; out may be y, and overlaps nothing else.  A row whose id is outside [0, n_adapters) gets
  * y[t] (-1: a request without an adapter).  Types: x fp32, y and out fp32; or x
- * of the weights' type, y and out of that type or fp32.  A x stays in fp32. */
+ * of the weights' type, y and out of that type or fp32.  Sums are fp32.  An fp32 x
+ * is used to 2^-22 of each value, and each value of A x to 2^-26 (bf16 weights, out
+ * fp32), 2^-23 (fp16 weights) or 2^-17 (bf16 weights and out): where y and the
+ * adapter's part cancel, that can be more than out's own rounding. */
 int moe_adapters_apply(const moe_adapters *set, const int32_t *ids, const void *x, int x_dtype, int64_t ld_x,
                        const void *y, int64_t ld_y, void *out, int out_dtype, int64_t ld_out, int n_tok,
                        void *stream);

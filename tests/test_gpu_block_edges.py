@@ -15,7 +15,8 @@ import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_gpu_block import BF16, F16, F32, H, U, check_route, close, randn, route_ref, router_logits  # noqa: E402
+from test_gpu_block import (BF16, F16, F32, H, U, check_route, close, d64, randn, route_ref,  # noqa: E402
+                            router_logits)
 
 pytestmark = pytest.mark.gpu
 
@@ -210,6 +211,40 @@ def test_combine_empty_pairs_add_nothing(h, weight):
     got = nm.combine(r, rows, pos.cuda(), w.masked_fill(empty, weight))
     assert torch.isfinite(want[0]).all() and torch.isfinite(want[1]).all()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- adapters ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("wt,parts", [(BF16, 2.0 ** -26), (F16, 2.0 ** -23)])
+@pytest.mark.parametrize("n", [40, 3000])     # both tile sizes
+def test_fp32_rows_keep_their_bits(n, wt, parts):
+    """One weight of 1 in A and in B: out is x as the two products see it.  hi is
+    off by half a step of 11 bits and lo is cut off at 11 bits below: 2^-22 of x;
+    A x = hi + lo has 23 bits, exact in fp32, and is split into parts that leave
+    out 2^-26 (three of bf16) or 2^-23 (two of fp16); their sum is exact."""
+    from moe_prefetch_b200 import AdapterSet
+    a, b = torch.zeros(1, 8, 64, dtype=wt).cuda(), torch.zeros(1, 16, 8, dtype=wt).cuda()
+    a[0, 3, 17], b[0, 5, 3] = 1.0, 1.0
+    x = torch.zeros(n, 64).cuda()
+    x[:, 17] = randn(n, seed=n)
+    out = AdapterSet(a, b)(x, torch.zeros(n, dtype=torch.int32, device="cuda"))
+    got, want = d64(out[:, 5]), d64(x[:, 17])
+    assert ((got - want).abs() <= (2.0 ** -22 + parts) * want.abs()).all(), ((got - want) / want).abs().max()
+
+
+@pytest.mark.parametrize("wt", [BF16, F16])
+def test_fp32_rows_of_the_largest_values(wt):
+    """Finite values up to the largest stay finite (2^-21 there)."""
+    from moe_prefetch_b200 import AdapterSet
+    a, b = torch.zeros(1, 1, 64, dtype=wt).cuda(), torch.zeros(1, 16, 1, dtype=wt).cuda()   # (rank 1: no 0 * inf)
+    a[0, 0, 1], b[0, 0, 0] = 2.0 ** -14, 1.0
+    v = torch.tensor([torch.finfo(F32).max, -torch.finfo(F32).max, 2.0 ** 127, 2.0 ** 127 - 2.0 ** 103, 3.4e38, math.inf, math.nan])
+    x = torch.zeros(7, 64)
+    x[:, 1] = v
+    out = d64(AdapterSet(a, b)(x.cuda(), torch.zeros(7, dtype=torch.int32, device="cuda"))[:, 0])
+    want = d64(v) * 2.0 ** -14
+    assert ((out - want).abs()[:5] <= (2.0 ** -21 + 2.0 ** -23) * want.abs()[:5]).all()
+    assert out[5] == math.inf and torch.isnan(out[6])
 
 
 # ---- a rule under the streaming lookahead ---------------------------------------------

@@ -550,7 +550,11 @@ __global__ void __launch_bounds__(AD_THREADS, NT > 8 ? 1 : 2) k_adapters(Adapter
                 for (int e = 0; e < 4; ++e) v[e] = low[j][e] * up;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    w[i] = ad_pack(v, TW());
+                    float c[4];   // v, but no finite value rounds to an infinite bf16
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        c[e] = !SCALED && i == 0 && fabsf(v[e]) < INFINITY ? fminf(fmaxf(v[e], -0x1.fep127f), 0x1.fep127f) : v[e];
+                    w[i] = ad_pack(c, TW());
                     float h[4];
                     uint32_t b0, b1;
                     pair32(w[i].x, b0, b1, TW());

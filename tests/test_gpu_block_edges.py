@@ -233,11 +233,12 @@ def test_fp32_rows_keep_their_bits(n, wt, parts):
 
 
 @pytest.mark.parametrize("wt", [BF16, F16])
-def test_fp32_rows_of_the_largest_values(wt):
-    """Finite values up to the largest stay finite (2^-21 there)."""
+@pytest.mark.parametrize("at", ["a", "b"])
+def test_fp32_rows_of_the_largest_values(wt, at):
+    """Finite values up to the largest stay finite (2^-21 there), in x and in A x."""
     from moe_prefetch_b200 import AdapterSet
     a, b = torch.zeros(1, 1, 64, dtype=wt).cuda(), torch.zeros(1, 16, 1, dtype=wt).cuda()   # (rank 1: no 0 * inf)
-    a[0, 0, 1], b[0, 0, 0] = 2.0 ** -14, 1.0
+    a[0, 0, 1], b[0, 0, 0] = (2.0 ** -14, 1.0) if at == "a" else (1.0, 2.0 ** -14)
     v = torch.tensor([torch.finfo(F32).max, -torch.finfo(F32).max, 2.0 ** 127, 2.0 ** 127 - 2.0 ** 103, 3.4e38, math.inf, math.nan])
     x = torch.zeros(7, 64)
     x[:, 1] = v

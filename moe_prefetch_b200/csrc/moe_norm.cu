@@ -567,7 +567,9 @@ static cudaError_t norm_launch(const NormArgs &a, int threads, cudaStream_t s) {
             (e = attr.need((const void *)k_block_norm<TR, TY, VEC, V, SRC, THREADS, S, EXACT>, (int)smem)) != cudaSuccess)
             return e;
     }
-    per_sm = std::min(16, std::max(1, per_sm));
+    // 65,536 narrow rows: 24 CTAs of a warp for 16-bit rows (64 of bf16 24.5 us, with 16 CTAs 32.8 and 12
+    // 30.5; beside fp32 r 31.7, 34.5, 38.8), 16 for fp32 (29.5; 24 CTAs 31.6)
+    per_sm = std::min(sizeof(TY) == 2 ? 24 : 16, std::max(1, per_sm));
     return launch_pdl(k_block_norm<TR, TY, VEC, V, SRC, THREADS, S, EXACT>, SRC ? a.n_tok : std::min(a.n_tok, sms * per_sm), threads,
                       smem, s, 0, a);
 }

@@ -396,3 +396,90 @@ def test_outputs_in_a_list_on_a_stream():
     s.synchronize()
     for got, want in ((out, rt(x)), (ro, nm(r, x)), (co, nm.combine(r, x, pos, w))):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- long strides, first calls, captured rules ------------------------------------------
+
+def test_rows_past_32_bits():
+    """Rows so far apart that their offsets pass 2^32 elements and bytes."""
+    from moe_prefetch_b200 import AdapterSet, BlockNorm, Routing
+    n, ld = 36, (1 << 27) + 64             # 36 * 2^27 elements of 16 bits: 9.7 GB, of which little is touched
+    big = torch.empty(n * ld, dtype=BF16, device="cuda").view(n, ld)
+    cols = [big[:, 64 * i:64 * (i + 1)] for i in range(5)]
+    r, y, x = (randn(n, 64, seed=s).to(BF16) for s in (1, 2, 3))
+    for c, v in zip(cols, (r, y, x)):
+        c.copy_(v)
+    rt = Routing(64, 4, score="sigmoid", bias=0.1 * randn(64, seed=4))
+    assert all(torch.equal(a, b) for a, b in zip(rt(cols[0]), rt(r)))
+    nm = BlockNorm(64, post=1 + 0.2 * randn(64, seed=5), pre=True)
+    want = nm(r, y)
+    nm(cols[0], cols[1], out=(cols[3], cols[4]))
+    assert torch.equal(cols[3], want[0]) and torch.equal(cols[4], want[1])
+    st = AdapterSet((randn(3, 8, 64, seed=6) / 8).to(BF16), randn(3, 64, 8, seed=7).to(BF16))
+    ids = (torch.arange(n, device="cuda") % 4 - 1).int()
+    want = st(x, ids, y)
+    assert torch.equal(st(cols[2], ids, cols[1], out=cols[3]), want)
+    assert torch.equal(st(cols[2], ids, cols[1], out=cols[1]), want)
+    f32 = big.view(F32)                    # combine: expert rows past 2^31 elements
+    rows = f32[:, 1024:1088]
+    rows.copy_(randn(n, 64, seed=8))
+    pos, w = torch.randperm(n, generator=torch.Generator().manual_seed(9)).int().view(n // 2, 2).cuda(), randn(n // 2, 2, seed=10)
+    got = nm.combine(r[:n // 2].float(), rows, pos, w)
+    want = nm.combine(r[:n // 2].float(), rows.contiguous(), pos, w)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+FIRST = """
+import torch
+from moe_prefetch_b200 import AdapterSet, BlockNorm, Routing
+torch.manual_seed(1)
+randn = lambda *s: torch.randn(*s, device="cuda")
+rt = Routing(128, 8, score="sigmoid", bias=randn(128), n_group=4, topk_group=2, group_top=2)
+nm, wide = BlockNorm(2048, post=randn(2048), pre=True), BlockNorm(16384, post=randn(16384), pre=True)
+st = AdapterSet(randn(4, 64, 2048).bfloat16() / 45, randn(4, 256, 64).bfloat16())
+lg, r, y, rw, yw, out = randn(300, 128), randn(300, 2048), randn(300, 2048), randn(3, 16384), randn(3, 16384), randn(300, 256)
+gate = randn(1, 1).expand(300, 1)
+ids = (torch.arange(300, device="cuda") % 5 - 1).int()
+pos, w = torch.randint(-1, 300, (300, 4), device="cuda").int(), randn(300, 4)
+call = lambda: [*rt(lg), *nm(r, y, gate=gate), *wide(rw, yw), *nm.combine(r, y, pos, w), st(y, ids, out)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = call()
+g.replay()
+want = call()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    """Nothing has to run before a capture: neither a kernel's first launch nor
+    its shared memory limit."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("n", [1, 6])
+def test_captured_layers_keep_their_rule(one_layer, n):
+    """A captured call of a layer with a rule gives the rule's results after
+    the layer has another."""
+    from moe_prefetch_b200 import Routing
+    x = randn(n, H, seed=1)
+    one_layer.set_routing(0, Routing(64, 8, score="sigmoid", n_group=8, topk_group=3, group_top=2, renorm=False))
+    try:
+        one_layer.block_forward(0, x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = one_layer.block_forward(0, x)
+        x.copy_(randn(n, H, seed=2))
+        want = one_layer.block_forward(0, x)
+    finally:
+        one_layer.set_routing(0, None)
+    g.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not torch.equal(one_layer.block_forward(0, x)[2], want[2])

@@ -573,8 +573,9 @@ int moe_route(const moe_route_cfg *cfg, const void *logits, int dtype, int64_t l
  * renormalisation again.  With the cache prior, delta is added to c of resident
  * experts after the groups are chosen.  The streaming lookahead ranks a layer's
  * experts by its rule (without prior or router adapters).  moe_decode has the
- * default rule built in and returns MOE_ERR_UNSUPPORTED while a layer has
- * another.  Synchronous. */
+ * default rule built in and returns MOE_ERR_UNSUPPORTED while a layer has one
+ * set.  A captured call keeps the rule of its capture, but reads the bias that was
+ * set last.  Synchronous. */
 int moe_set_routing(moe_ctx *ctx, int layer, const moe_route_cfg *cfg, const float *bias);
 
 #define MOE_GATE_NONE    0
@@ -588,7 +589,8 @@ int moe_set_routing(moe_ctx *ctx, int layer, const moe_route_cfg *cfg, const flo
  *   z  = y / sqrt(mean(y^2) + eps) * (post + weight_offset)   (z = y without post)
  *   r' = r + scale * act(gate) * z
  *   x  = r' / sqrt(mean(r'^2) + eps) * (pre + weight_offset)  (factor 1 without pre)
- * in fp32, each of r' and x rounded once to its type (x from the unrounded r').
+ * in fp32, each of r' and x rounded once to its type (x from the unrounded r'); a
+ * sigmoid is off by up to 4 ulp, and 0 below 2^-126.
  * post / pre are fp32 [n_embd] or NULL; weight_offset 1 for weights stored
  * around 0.  n_embd <= 16384.  Rows of 16-byte-aligned pointers and strides with
  * n_embd % 8 == 0 take vector loads; others are accepted. */

@@ -171,7 +171,7 @@ cudaError_t launch_route_one(const RouteSpec &sp, const float *logits, int32_t *
 // ---- the norms around a block (moe_norm.cu) ---------------------------------
 
 enum { NORM_GATE_NONE = 0, NORM_GATE_TOKEN = 1, NORM_GATE_CHANNEL = 2, NORM_GATE_FULL = 3 };
-constexpr int NORM_MAX_EMBD = 16384;   // 1024 threads of 16 values
+constexpr int NORM_MAX_EMBD = 16384;   // a row in fp32 takes 64 KB of shared memory (k_block_norm_wide)
 
 struct NormArgs {
     int n_tok, n_embd;

@@ -159,9 +159,9 @@ __host__ __device__ __forceinline__ int norm_row_bytes(const NormArgs &a) {
 // barrier): the kernel is bound by memory, and S - 1 rows are on their way while
 // one is in its two sums.
 // CTAs of 256 threads per SM: four, or three with more registers where that is
-// faster (8,192 rows of 2,048, bf16 beside an fp32 residual with a full gate: 40.0
-// us with three, 42.9 with four; all bf16: 26.0 and 32.9; bf16 rows of 1,537: 84 and
-// 142).
+// faster (8,192 rows of 2,048, bf16 beside an fp32 residual with a full gate: 38.7
+// us with three, 42.4 with four; all bf16, no gate: 27.0 and 29.1; 10,915 bf16 rows of
+// 1,537: 84 and 131; fp32 rows of 1,000 are the other way: 45.8 with four, 50.9 with three).
 template <typename TR, int VEC, int SRC, int THREADS, bool EXACT> constexpr int norm_ctas() {
     return THREADS > 256 ? 1 : SRC == 0 && (EXACT || VEC == 1 || sizeof(TR) == 2) ? 3 : 4;
 }
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, norm_ctas<TR, VEC, SRC, THREADS, EXAC
     bool in_[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) in_[c] = at(c) < H;
-    // whether the thread has chunk c: all of them (EXACT: 40.0 us of the case above, 45.7 without),
+    // whether the thread has chunk c: all of them (EXACT: 38.7 us of the case above, 44.5 without),
     // compared anew where registers are short, else kept
     auto in = [&](int c) {
         if constexpr (EXACT) return true;   // every thread has all its chunks

@@ -72,8 +72,7 @@ __device__ __forceinline__ uint64_t route_key(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-// Largest value of the warp, by shuffles: ptxas 12.9 miscompiles the integer
-// reduction of order-preserving keys turned back into a float.
+// Largest value of the warp, by shuffles.
 __device__ __forceinline__ float route_warp_max(float v) {
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(MOE_FULL, v, off));

@@ -343,8 +343,8 @@ __device__ __forceinline__ float route_load(const __half *p) { return __half2flo
 // experts.
 //
 // The weights are formed in 32 bits (expf 4 u with the rounding of l - mx taken
-// back, k - 1 additions in five levels, two divisions, scale: below 20 u); where
-// their sum is so small that scores may have underflowed, in 64 bits.
+// back, k - 1 additions in five levels, two divisions, scale: below 20 u);
+// renormalised ones in 64 bits where a score underflows or their sum is very small.
 template <int J, typename T>
 __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s, const int32_t *table, int ns,
                                                float delta, bool prior, const int32_t *pub, int lane, int &id_r,
@@ -412,7 +412,10 @@ __device__ __forceinline__ void route_warp_row(const T *row, const RouteSpec &s,
         if (v > 0.0f) v = fmaf(v, rest, v);                 // (d may be -inf)
     }
     if (s.renorm) total = warp_sum(lane < s.k ? v : 0.0f);
-    if (s.renorm && total < 1e-20f) {
+    // a score other than 0 below fp32's normal range: its share of a small sum may not be small
+    const bool low = __any_sync(MOE_FULL, v < 0x1p-126f && l_r > -INFINITY);
+    if (low && s.sigmoid && !s.renorm && l_r < -80.0f) v = expf(l_r);   // (e^80 may be too large, 1 + e^-80 is 1)
+    if (s.renorm && (low || total < 1e-20f)) {
         double x = 0.0, sum;
         if (lane < s.k)
             x = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l_r)) : mx > -INFINITY ? exp((double)l_r - (double)mx) : 0.0;

@@ -125,6 +125,32 @@ def test_a_layer_takes_a_masked_rule():
         st.close()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("scale", [1.0, 1.5])
+def test_weights_of_far_logits(score, renorm, scale):
+    """Scores that underflow in 32 bits beside a small sum: every weight is
+    within 32 u of its value, or two steps of the smallest fp32 (one rounding
+    there, and one of its product with the scale)."""
+    from moe_prefetch_b200 import Routing
+    E, k = 64, 8
+    x = torch.full((40, E), -300.0)
+    for t in range(40):        # the bias decides: the chosen are 40 to 103 below the largest, or below 0
+        x[t, :k] = -40.0 - 1.6 * t - 6.0 * torch.arange(k)
+        x[t, k - 1] = -103.0
+    x[:, E - 1] = 0.0
+    x[5, :k] = -20.0 * torch.arange(k) - 10.0
+    x[6, :k] = torch.tensor([-87.0, -88.5, -88.9, -90.0, -95.0, -100.0, -103.0, -110.0])
+    b = torch.zeros(E)
+    b[:k] = 4.0 + torch.arange(k) / 16
+    x, b = x.cuda(), b.cuda()
+    ids, w = Routing(E, k, score=score, bias=b, renorm=renorm, scale=scale)(x)
+    rid, rw = route_ref(x, k, score=score, bias=b, renorm=renorm, scale=scale)
+    assert torch.equal(ids.long().cpu(), rid)
+    err = (d64(w) - rw).abs()
+    assert (err <= 32 * U * rw + 2 * 2.0 ** -149).all(), (err / rw.clamp(min=1e-300)).max()
+
+
 # ---- outputs beside and over inputs ---------------------------------------------------
 
 def test_outputs_between_the_rows_of_inputs():

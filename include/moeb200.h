@@ -547,7 +547,8 @@ int moe_synth_f32(float *y, int64_t n, uint64_t seed, float sigma, void *stream)
  * last, where fewer than k others are left, and a group's sum of two leaves it
  * out.  The
  * comparison is exact: it goes by the logits where c falls with them, else by
- * c in 64 bits, so that no rounding to 32 bits decides between experts.
+ * c in 64 bits, so that no rounding to 32 bits decides between experts (a score
+ * below 2^-1022 may be 0).
  * Limits: n_expert <= 512, k <= 32, n_group <= 32, a divisor of n_expert;
  * k <= topk_group * n_expert / n_group.  The reference routes by softmax,
  * top-k and renormalisation alone (context of patches/0007:101-128), which is

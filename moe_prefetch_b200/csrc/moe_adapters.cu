@@ -26,7 +26,7 @@
 // Measured: 4,096 prompt tokens, 8 adapters of rank 64, 2048 -> 2048, all bf16: 28.6
 // us (54 MB, 8.3 us of a measured copy; finding the tile 3.6 us, first product 7,
 // the sums' exchange 5, second product 10; the tensor pipe is 24 % busy).  32
-// requests, 16 adapters of rank 16, fp32: 7.7 us; one token, rank 8, 2048 -> 128:
+// requests, 16 adapters of rank 16, fp32: 7.8 us; one token, rank 8, 2048 -> 128:
 // 5.6 us.
 #include "moe_kernels.h"
 

@@ -7,9 +7,9 @@ namespace moe {
 
 // grid ceil(n_tok / ROUTE_WARPS); block ROUTE_WARPS warps.  A warp per token: a
 // token's experts fit its lanes' registers, and no barrier is needed.  Bound by
-// integer instructions (the ALU pipe is 63 % busy): 8,192 tokens of 256 experts in
-// four groups, sigmoid and bias, bf16, take 15.1 us (0.7 us of memory traffic);
-// one token of 128 experts takes 2.1 us, the launch included.
+// integer instructions (the ALU pipe is 64 % busy): 8,192 tokens of 256 experts in
+// four groups, sigmoid and bias, bf16, take 15.3 us (0.7 us of memory traffic);
+// one token of 128 experts takes 2.2 us, the launch included.
 template <typename T, int J>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
     k_route(RouteSpec spec, const T *__restrict__ logits, int64_t ld, int n_tok, int32_t *__restrict__ ids,

@@ -1869,7 +1869,9 @@ static NormArgs norm_args(const moe_norm &n, int n_tok) {
 // Whether an output of the norm meets what it may not: r_out and x may each be
 // r, y rows, a full gate or add (every thread reads its part of a row before it
 // writes there), and meet nothing else.
-static bool norm_meets(const NormArgs &a, int dt_r, int dt_y) {
+// What else a call writes before it reads the norm's inputs (`before`, of
+// moe_block_forward) meets none of them.
+static bool norm_meets(const NormArgs &a, int dt_r, int dt_y, std::initializer_list<Rows> before = {}) {
     const int64_t n = a.n_tok, h = a.n_embd, sr = dtype_size(dt_r), sy = dtype_size(dt_y);
     const Rows none{};
     const Rows r = {a.r, n, h * sr, a.ld_r * sr}, add = {a.add, n, h * 4, h * 4};
@@ -1882,6 +1884,8 @@ static bool norm_meets(const NormArgs &a, int dt_r, int dt_y) {
     const Rows pos = flat(a.pos, 4 * n * a.k), w = flat(a.w, 4 * n * a.k), po = flat(a.post, 4 * h), pr = flat(a.pre, 4 * h);
     for (const Rows &o : {ro, x})
         if (out_meets(o, {r, a.pos ? none : y, gate, add}, {a.pos ? y : none, g1, pos, w, po, pr})) return true;
+    for (const Rows &o : before)
+        if (out_meets(o, {}, {r, gate, g1, po, pr, ro, x})) return true;
     return rows_meet(ro, x);
 }
 
@@ -2024,17 +2028,17 @@ extern "C" int moe_block_forward(moe_ctx *c, int layer, const float *x, int n_to
         const int64_t n = n_tok, k = g.n_used;
         const Rows rx = {x, n, 4 * H, 4 * H}, ry = {y, n, 4 * H, 4 * H}, ri = flat(ids, 4 * n * k), rw = flat(w, 4 * n * k);
         const Rows ra_ids = flat(ra || la ? b->adapter_ids : nullptr, 4 * n);
-        Rows ro{}, xo{}, rr{};
+        Rows ro{}, xo{};
         bool bad = out_meets(ry, {}, {rx, ri, rw, ra_ids});
         if (b->norm) {
             NormArgs a = norm_args(*b->norm, n_tok);
             a.r = b->r; a.r_out = b->r_out; a.x = b->x_out;
             a.ld_r = a.ld_ro = a.ld_x = H;
-            rr = {b->r, n, 4 * H, 4 * H}; ro = {b->r_out, n, 4 * H, 4 * H}; xo = {b->x_out, n, 4 * H, 4 * H};
-            bad = norm_meets(a, MOE_DTYPE_F32, MOE_DTYPE_F32) || out_meets(ro, {rx}, {ri, rw, ra_ids}) ||
-                  out_meets(xo, {rx}, {ri, rw, ra_ids});
+            ro = {b->r_out, n, 4 * H, 4 * H}; xo = {b->x_out, n, 4 * H, 4 * H};
+            bad = norm_meets(a, MOE_DTYPE_F32, MOE_DTYPE_F32, {ri, rw}) || out_meets(ro, {rx}, {ra_ids}) ||
+                  out_meets(xo, {rx}, {ra_ids});
         }
-        for (const Rows &o : {ri, rw}) bad = bad || out_meets(o, {}, {rx, rr, ra_ids});
+        for (const Rows &o : {ri, rw}) bad = bad || out_meets(o, {}, {rx, ra_ids});
         bad = bad || rows_meet(ri, rw);
         for (const moe_adapters *s : {ra, la})
             if (s)

@@ -198,10 +198,10 @@ def test_block_refuses_overlaps():
         ids, w = torch.zeros(n, 8, dtype=torch.int32, device="cuda"), torch.zeros(n, 8, device="cuda")
         nm = BlockNorm(H, pre=True)
 
-        def rc(x, y=None, r=None, ro=None, xo=None, i=ids.data_ptr(), ww=w.data_ptr()):
+        def rc(x, y=None, r=None, ro=None, xo=None, i=ids.data_ptr(), ww=w.data_ptr(), gate=None):
             b = _lib.MoeBlock()
             if y is None:
-                b.norm, b.r, b.r_out, b.x_out = C.pointer(nm.nm), r, ro, xo
+                b.norm, b.r, b.r_out, b.x_out = C.pointer(nm.with_gate(gate, n, F32, ids.device)), r, ro, xo
             return st.lib.moe_block_forward(st.ctx, 0, x, n, C.byref(b), y, C.c_void_p(i), C.c_void_p(ww), 0, None)
 
         assert rc(part(0), y=part(1)) == 0
@@ -210,7 +210,9 @@ def test_block_refuses_overlaps():
         for bad in (dict(y=part(0)), dict(y=part(0, 64)), dict(y=part(1), i=w.data_ptr()), dict(y=part(1), i=buf.data_ptr()),
                     dict(y=part(1), ww=buf.data_ptr() + 4 * n * H), dict(r=part(1), ro=part(1, 8), xo=part(3)),
                     dict(r=part(1), ro=part(2), xo=part(2, 8)), dict(r=part(1), ro=part(2), xo=part(0, 4)),
-                    dict(r=part(1), ro=part(2), xo=C.c_void_p(ids.data_ptr()))):
+                    dict(r=part(1), ro=part(2), xo=C.c_void_p(ids.data_ptr())),
+                    dict(r=part(1), ro=part(2), xo=part(3), i=buf.data_ptr() + 4 * n * H),
+                    dict(r=part(1), ro=part(2), xo=part(3), gate=w[:, :1])):
             assert rc(part(0), **bad) == -1, bad
         torch.cuda.synchronize()
     finally:

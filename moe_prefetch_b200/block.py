@@ -315,7 +315,9 @@ class AdapterSet:
 
     ``adapters(x, ids, y)`` -> y[t] + scale[i] * b[i] (a[i] x[t]), i = ids[t];
     a row with id -1 (or any id outside the set) keeps y[t].  The weights are
-    laid out once, here; a later change of a or b is not seen."""
+    laid out once, here, on the current stream; a later change of a or b is not
+    seen.  How many bits of x and of A x the products use stands at
+    moe_adapters_apply."""
 
     MAX_RANK = 128
 
